@@ -53,6 +53,15 @@ def _load():
     lib.b200moe_ep_unpack.argtypes = [vp, vp, i, vp, vp, vp, vp, vp]
     lib.b200moe_set_wait_limit_ns.argtypes = [vp, C.c_ulonglong]
     lib.b200moe_quantize_1x128.argtypes = [vp, i, i, vp, vp, vp]
+    lib.b200moe_sort_workspace_bytes.argtypes = [i, i, i, C.POINTER(sz)]
+    lib.b200moe_sort_tokens.argtypes = [vp, i, i, i, i, i, i, vp, vp, vp, vp, sz, vp]
+    lib.b200moe_permute.argtypes = [vp, i, vp, vp, vp, i, i, i, i, i, vp, vp]
+    lib.b200moe_restore_1x128.argtypes = [vp, vp, i, vp, vp, vp, i, i, i, i, i, vp, vp]
+    lib.b200moe_combine.argtypes = [vp, i, vp, vp, i, i, i, i, vp, vp]
+    lib.b200moe_combine_backward.argtypes = [vp, vp, i, vp, vp, vp, vp, i, i, i, i, i, vp, vp, vp]
+    lib.b200moe_swiglu_save.argtypes = [vp, i, vp, i, i, vp, vp, vp, vp]
+    lib.b200moe_swiglu_backward.argtypes = [vp, vp, vp, i, vp, i, i, vp, vp, vp]
+    lib.b200moe_route_backward.argtypes = [vp, vp, vp, vp, i, i, i, f, i, vp, vp]
     lib.b200moe_status.argtypes = [vp, vp, vp, C.POINTER(i)]
     lib.b200moe_set_fused_combine.argtypes = [vp, i]
     lib.b200moe_set_tma_gather.argtypes = [vp, i]
@@ -69,7 +78,9 @@ def _load():
     for name in ("create", "destroy", "workspace_bytes", "workspace_layout", "forward", "route",
                  "forward_routed", "status", "set_fused_combine", "set_tma_gather", "set_token_tile", "launches_per_forward", "launches_routed", "launches_routed_slots", "num_sms", "profile_enable",
                  "profile_read", "permute_noalloc", "ep_combine", "ep_row_bytes", "ep_pack", "ep_unpack", "ep_push", "ep_barrier", "ep_unpack_slots",
-                 "ep_return", "ep_combine_slots", "forward_routed_slots", "quantize_1x128", "set_wait_limit_ns"):
+                 "ep_return", "ep_combine_slots", "forward_routed_slots", "quantize_1x128", "set_wait_limit_ns",
+                 "sort_workspace_bytes", "sort_tokens", "permute", "restore_1x128", "combine", "combine_backward", "swiglu_save",
+                 "swiglu_backward", "route_backward"):
         getattr(lib, "b200moe_" + name).restype = i
     return lib
 

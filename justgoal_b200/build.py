@@ -12,8 +12,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200moe.so")
-SOURCES = ["b200moe.cu"]
-HEADERS = ["common.cuh", "routing.cuh", "permute.cuh", "front.cuh", "ep_p2p.cuh", "gemm.cuh", "gemm_pair.cuh", "quant.cuh", os.path.join("..", "..", "include", "b200moe.h")]
+SOURCES = ["b200moe.cu", "train.cu"]
+HEADERS = ["common.cuh", "routing.cuh", "permute.cuh", "front.cuh", "ep_p2p.cuh", "gemm.cuh", "gemm_pair.cuh", "quant.cuh", "order.cuh",
+           "swiglu.cuh", "route_grad.cuh", os.path.join("..", "..", "include", "b200moe.h"),
+           os.path.join("..", "..", "include", "b200moe_train.h")]
 
 
 def _nvcc() -> str:
@@ -36,7 +38,7 @@ def build(force: bool = False, verbose: bool = False, out: str = None) -> str:
     if out is None and not force and not needs_build():
         return LIB
     cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
-           "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(HERE, "..", "include"),
+           "-shared", "-Xcompiler", "-fPIC", "--threads", "0", "-I", os.path.join(HERE, "..", "include"),
            "-o", out or LIB] + [os.path.join(CSRC, s) for s in SOURCES]
     extra = os.environ.get("B200MOE_NVCC_FLAGS")      # e.g. -DB200MOE_ENABLE_KLOG for the per-K-block log
     if extra:

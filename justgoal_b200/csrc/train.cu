@@ -1,0 +1,212 @@
+// Host side of the training operators of libb200moe (token order, 8-bit SwiGLU copies, router gradient): argument checks and
+// launches for the C ABI declared in include/b200moe_train.h.  Nothing here keeps state: every call works on its arguments alone, on
+// the current device and the caller's stream, so calls on different streams share nothing.
+#include <cuda_runtime.h>
+
+#include "b200moe_train.h"
+#include "order.cuh"
+#include "route_grad.cuh"
+#include "swiglu.cuh"
+
+using namespace b200moe;
+
+namespace {
+
+// Launched with programmatic stream serialization: the start hides under the tail of the kernel before it, and every kernel waits for
+// that one to complete before it reads or writes global memory.
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, int block, void* stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+}
+
+int sm_count() {
+    const int n = b200moe_num_sms();
+    return n > 0 ? n : 148;
+}
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+bool known_type(int type) { return type == B200MOE_TYPE_BF16 || type == B200MOE_TYPE_FP16 || type == B200MOE_TYPE_FP32; }
+int type_bytes(int type) { return type == B200MOE_TYPE_FP32 ? 4 : 2; }
+
+int sort_ctas(int n) { return n <= SORT_ONE ? 1 : (n + SORT_SLICE - 1) / SORT_SLICE; }
+
+bool bad_picks(int T, int top_k) { return T < 0 || top_k < 1 || top_k > ORDER_MAX_PICKS || (long long)T * top_k > (1ll << 30); }
+
+// The sizes and tables that the row kernels share
+int check_order(const OrderParams& o, int H) {
+    if (bad_picks(o.T, o.top_k) || o.num_local < 1 || o.num_local > ORDER_MAX_LOCAL || o.num_rows < 0 || H <= 0 || H % 128) return B200MOE_E_BADARG;
+    return 0;
+}
+
+// Grid of a kernel whose warps take one token each: up to eight CTAs of eight warps per SM; few tokens share a token's columns among
+// gridDim.y CTAs, `units` steps of a lane being what there is to share.
+dim3 warp_grid(int T, int units) {
+    const int sms = sm_count();
+    const int x = max(1, min((T + 7) / 8, sms * 8));
+    int y = 1;
+    while (x * y < sms * 2 && y * 64 <= units) y *= 2;
+    return dim3(x, y);
+}
+
+template <typename T>
+int combine_rows(const OrderParams& o, const void* rows, const float* w, void* out, int H, void* stream) {
+    return launch(combine_rows_kernel<T>, warp_grid(o.T, H * (int)sizeof(T) / 16), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
+}
+
+template <typename T>
+int combine_grad(const OrderParams& o, const void* d_out, const void* rows, const float* w, void* d_rows, float* d_w, int H, void* stream) {
+    const int units = H * (int)sizeof(T) / 16;
+    const int block = units >= 256 ? 256 : units >= 128 ? 128 : units >= 64 ? 64 : 32;
+    const int grid = min(max(o.T, 1), sm_count() * (2048 / block));
+    return launch(combine_grad_kernel<T>, dim3(grid), block, stream, o, static_cast<const T*>(d_out), static_cast<const T*>(rows), w,
+                  static_cast<T*>(d_rows), d_w, H);
+}
+
+template <typename T>
+int restore_rows(const OrderParams& o, const void* q, const float* scale, void* rows, int H, void* stream) {
+    return launch(restore_rows_kernel<T>, warp_grid(o.T, H / 16), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
+}
+
+// Block of a CTA of the SwiGLU kernels: eight rows (a sector of scales), more where rows have few groups
+void swiglu_block(int rows, int I, int& rsh, int& gpc, dim3& grid) {
+    const int groups = I >> 7, parts = (groups + 63) / 64;
+    gpc = (groups + parts - 1) / parts;
+    rsh = 3;
+    while ((gpc << rsh) < SWIGLU_TURN) ++rsh;
+    while (rsh > 0 && (long long)((rows + (1 << rsh) - 1) >> rsh) * parts < 2ll * sm_count()) --rsh;
+    grid = dim3((rows + (1 << rsh) - 1) >> rsh, (groups + gpc - 1) / gpc);
+}
+
+template <typename T>
+int swiglu_save(const void* x, const int32_t* used, int rows, int I, void* act, void* q, float* scale, void* stream) {
+    int rsh, gpc;
+    dim3 grid;
+    swiglu_block(rows, I, rsh, gpc, grid);
+    return launch(swiglu_save_kernel<T>, grid, SWIGLU_THREADS, stream, static_cast<const T*>(x), used, rows, I, rsh, gpc, static_cast<T*>(act),
+                  static_cast<uint8_t*>(q), scale);
+}
+
+template <typename T>
+int swiglu_grad(const void* q, const float* scale, const void* d_act, const int32_t* used, int rows, int I, void* d_x, void* act, void* stream) {
+    int rsh, gpc;
+    dim3 grid;
+    swiglu_block(rows, I, rsh, gpc, grid);
+    return launch(act ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>, grid, SWIGLU_THREADS, stream, static_cast<const uint8_t*>(q), scale,
+                  static_cast<const T*>(d_act), used, rows, I, rsh, gpc, static_cast<T*>(d_x), static_cast<T*>(act));
+}
+
+}  // namespace
+
+#define BY_TYPE(call) (type == B200MOE_TYPE_BF16 ? call<__nv_bfloat16> : type == B200MOE_TYPE_FP16 ? call<__half> : call<float>)
+
+extern "C" {
+
+int b200moe_sort_workspace_bytes(int T, int top_k, int num_local, size_t* bytes) {
+    if (!bytes || bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL) return B200MOE_E_BADARG;
+    const int ctas = sort_ctas(T * top_k);
+    *bytes = ctas > 1 ? (size_t)ctas * num_local * sizeof(int) : 0;
+    return 0;
+}
+
+int b200moe_sort_tokens(const int32_t* topk_idx, int T, int top_k, int num_local, int local_offset, int align, int max_rows,
+                        int32_t* expert_row0, int32_t* row_pair, int32_t* pair_row, void* workspace, size_t workspace_bytes, void* stream) {
+    if (bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL || align < 1 || align > 128 || (align & (align - 1)) || max_rows < 0)
+        return B200MOE_E_BADARG;
+    if (!expert_row0 || (max_rows && !row_pair) || (T && (!topk_idx || !pair_row))) return B200MOE_E_BADARG;
+    SortParams p;
+    p.topk_idx = topk_idx; p.n = T * top_k; p.num_local = num_local; p.local_offset = local_offset; p.align = align; p.max_rows = max_rows;
+    p.slices = static_cast<int*>(workspace); p.expert_row0 = expert_row0; p.row_pair = row_pair; p.pair_row = pair_row;
+    const int ctas = sort_ctas(p.n);
+    if (ctas == 1) return launch(sort_one_kernel, dim3(1), SORT_THREADS, stream, p);
+    if (!workspace || misaligned(workspace, 4) || workspace_bytes < (size_t)ctas * num_local * sizeof(int)) return B200MOE_E_WORKSPACE;
+    const int rc = launch(sort_count_kernel, dim3(ctas), SORT_THREADS, stream, p);
+    return rc ? rc : launch(sort_place_kernel, dim3(ctas), SORT_THREADS, stream, p);
+}
+
+int b200moe_permute(const void* x, int type, const int32_t* expert_row0, const int32_t* row_pair, const int32_t* pair_row, int T, int top_k,
+                    int num_local, int hidden, int num_rows, void* rows, void* stream) {
+    const OrderParams o = {expert_row0, row_pair, pair_row, T, top_k, num_local, num_rows};
+    if (!known_type(type) || check_order(o, hidden)) return B200MOE_E_BADARG;
+    if (num_rows == 0) return 0;
+    if (!expert_row0 || !row_pair || !rows || (T && (!x || !pair_row)) || misaligned(x, 32) || misaligned(rows, 32)) return B200MOE_E_BADARG;
+    const int units = hidden * type_bytes(type) / 32;
+    return launch(permute_rows_kernel, warp_grid(T, units), 256, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
+}
+
+int b200moe_restore_1x128(const void* q, const float* scale, int type, const int32_t* expert_row0, const int32_t* row_pair, const int32_t* pair_row,
+                          int T, int top_k, int num_local, int hidden, int num_rows, void* rows, void* stream) {
+    const OrderParams o = {expert_row0, row_pair, pair_row, T, top_k, num_local, num_rows};
+    if (!known_type(type) || misaligned(q, 16) || misaligned(rows, 32)) return B200MOE_E_BADARG;
+    if (pair_row || row_pair || expert_row0) {
+        if (check_order(o, hidden)) return B200MOE_E_BADARG;
+        if (num_rows == 0) return 0;
+        if (!expert_row0 || !row_pair || !rows || (T && (!q || !scale || !pair_row))) return B200MOE_E_BADARG;
+    } else {
+        if (T < 0 || hidden <= 0 || hidden % 128) return B200MOE_E_BADARG;
+        if (T == 0) return 0;
+        if (!q || !scale || !rows) return B200MOE_E_BADARG;
+    }
+    return BY_TYPE(restore_rows)(o, q, scale, rows, hidden, stream);
+}
+
+int b200moe_combine(const void* rows, int type, const float* topk_w, const int32_t* pair_row, int T, int top_k, int hidden, int num_rows, void* out,
+                    void* stream) {
+    const OrderParams o = {nullptr, nullptr, pair_row, T, top_k, 1, num_rows};
+    if (!known_type(type) || check_order(o, hidden)) return B200MOE_E_BADARG;
+    if (T == 0) return 0;
+    if (!pair_row || !out || (num_rows && !rows) || misaligned(rows, 32) || misaligned(out, 32)) return B200MOE_E_BADARG;
+    return BY_TYPE(combine_rows)(o, rows, topk_w, out, hidden, stream);
+}
+
+int b200moe_combine_backward(const void* grad_out, const void* rows, int type, const float* topk_w, const int32_t* expert_row0, const int32_t* row_pair,
+                             const int32_t* pair_row, int T, int top_k, int num_local, int hidden, int num_rows, void* grad_rows, float* grad_w,
+                             void* stream) {
+    const OrderParams o = {expert_row0, row_pair, pair_row, T, top_k, num_local, num_rows};
+    if (!known_type(type) || check_order(o, hidden)) return B200MOE_E_BADARG;
+    if (T == 0 && num_rows == 0) return 0;
+    if (!expert_row0 || (num_rows && (!row_pair || !rows || !grad_rows)) || (T && (!grad_out || !topk_w || !pair_row || !grad_w))) return B200MOE_E_BADARG;
+    if (misaligned(grad_out, 32) || misaligned(rows, 32) || misaligned(grad_rows, 32)) return B200MOE_E_BADARG;
+    return BY_TYPE(combine_grad)(o, grad_out, rows, topk_w, grad_rows, grad_w, hidden, stream);
+}
+
+int b200moe_swiglu_save(const void* gemm1_rows, int type, const int32_t* used_rows, int num_rows, int intermediate, void* act, void* q, float* scale,
+                        void* stream) {
+    if (!known_type(type) || num_rows < 0 || intermediate <= 0 || intermediate % 128 || intermediate > (1 << 20)) return B200MOE_E_BADARG;
+    if (num_rows == 0) return 0;
+    if (!gemm1_rows || !act || !q || !scale || misaligned(gemm1_rows, 32) || misaligned(act, 32) || misaligned(q, 16)) return B200MOE_E_BADARG;
+    return BY_TYPE(swiglu_save)(gemm1_rows, used_rows, num_rows, intermediate, act, q, scale, stream);
+}
+
+int b200moe_swiglu_backward(const void* q, const float* scale, const void* grad_act, int type, const int32_t* used_rows, int num_rows, int intermediate,
+                            void* grad_gemm1_rows, void* act, void* stream) {
+    if (!known_type(type) || num_rows < 0 || intermediate <= 0 || intermediate % 128 || intermediate > (1 << 20)) return B200MOE_E_BADARG;
+    if (num_rows == 0) return 0;
+    if (!q || !scale || !grad_act || !grad_gemm1_rows) return B200MOE_E_BADARG;
+    if (misaligned(q, 16) || misaligned(grad_act, 32) || misaligned(grad_gemm1_rows, 32) || misaligned(act, 32)) return B200MOE_E_BADARG;
+    return BY_TYPE(swiglu_grad)(q, scale, grad_act, used_rows, num_rows, intermediate, grad_gemm1_rows, act, stream);
+}
+
+int b200moe_route_backward(const float* routing_logits, const void* routing_bias, const int32_t* topk_idx, const float* grad_w, int T, int num_experts,
+                           int top_k, float routed_scaling_factor, int routing_mode, float* grad_logits, void* stream) {
+    if (bad_picks(T, top_k) || num_experts < 32 || num_experts > 128 * ROUTE_GRAD_COLS || num_experts % 32 || top_k > num_experts) return B200MOE_E_BADARG;
+    if (routing_mode < 0 || routing_mode >= RG_COUNT || (routing_mode == RG_LLAMA4 && top_k != 1)) return B200MOE_E_BADARG;
+    if (T == 0) return 0;
+    if (!routing_logits || !topk_idx || !grad_w || !grad_logits || misaligned(routing_logits, 16) || misaligned(grad_logits, 16)) return B200MOE_E_BADARG;
+    const RouteGradParams p = {routing_logits, static_cast<const __nv_bfloat16*>(routing_bias), topk_idx, grad_w, grad_logits, T, num_experts, top_k,
+                               routed_scaling_factor};
+    auto* kern = routing_mode == RG_DEEPSEEK  ? route_grad_kernel<RG_DEEPSEEK>
+                 : routing_mode == RG_DEFAULT ? route_grad_kernel<RG_DEFAULT>
+                 : routing_mode == RG_LLAMA4  ? route_grad_kernel<RG_LLAMA4>
+                 : routing_mode == RG_TOPK    ? route_grad_kernel<RG_TOPK>
+                                              : route_grad_kernel<RG_RENORMALIZE>;
+    return launch(kern, dim3((T + 7) / 8), 256, stream, p);
+}
+
+}  // extern "C"

@@ -1,0 +1,318 @@
+"""Training operators around the layer's GEMMs: token order, 8-bit activation copies, router gradient.
+
+    idx, w = layer.route(logits, bias, factor)
+    order = sort_tokens(idx, E_local, offset)                     # expert-sorted tables
+    x_rows = permute(x, order)                                    # token rows in expert order      -> GEMM1 per expert
+    act, q, scale = swiglu_save(g_rows, order.expert_row0)        # activation, 8-bit copy of g     -> GEMM2 per expert
+    out = combine(y_rows, w, order)                               # weighted sum back per token
+
+and in the backward pass, with what GEMM2's and GEMM1's gradients give between them,
+
+    grad_y, grad_w = combine_backward(grad_out, y_rows, w, order)
+    grad_g, act = swiglu_backward(q, scale, grad_act, order.expert_row0)      # act again: it need not be kept
+    x_rows = restore_1x128(xq, xscale, order)                     # or permute(x, order): GEMM1's input rows again
+    grad_x = permute_backward(grad_rows, order)
+    grad_logits = route_backward(logits, bias, idx, grad_w, factor, mode)
+
+Every call runs on the current stream of its tensors' device, whichever device is current, allocates nothing but its outputs (and a table of
+counts in `sort_tokens`), keeps nothing, and can be captured into a CUDA graph.  Row tensors are bf16, fp16 or fp32; tensors that are not contiguous, or do
+not start at a 32-byte boundary, are copied first (`out` tensors are refused).  Row tensors have room for `order.row_pair.numel()` rows:
+`permute`, `restore_1x128`, `combine_backward` and the SwiGLU pair write the rows in use, padding of the segments included (as zeros), and leave
+those behind `expert_row0[-1]` as they were (unset where the call makes the tensor).  The gradients are plain functions: autograd does not record these calls.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .inputs import ROUTING_DS
+from .main import _raw_stream
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ALIGN = 32
+
+
+class TokenOrder(NamedTuple):
+    """Tables of `sort_tokens`, int32: first row of each local expert [E_local + 1], pair of each row [max_rows] and row of
+    each pair [T, top_k]; -1 where there is none."""
+    expert_row0: torch.Tensor
+    row_pair: torch.Tensor
+    pair_row: torch.Tensor
+
+
+def _call(name, device, *args):
+    fn = getattr(_lib.lib, name)
+    if torch.cuda.current_device() == device:
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _device(t, name):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _in(t, name, device, dtype, shape=None, align=4):
+    """An input as the library takes it: checked, contiguous, aligned."""
+    if t.dtype is not dtype or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name}: expected {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is not on cuda:{device}")
+    if not t.is_contiguous() or t.data_ptr() % align:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _out(t, name, device, dtype, shape, align=_ALIGN):
+    """An output: made here, or the caller's if it is of the form that can be written in place."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous() or t.data_ptr() % align:
+        raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on cuda:{device} that starts at a multiple of {align} bytes")
+    return t
+
+
+def _overlap(a, b):
+    return a.numel() and b.numel() and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def _apart(out, name, *inputs):
+    if any(_overlap(out, t) for t in inputs):
+        raise ValueError(f"{name} must not share memory with an input or another output")
+
+
+def _rows_type(t, name):
+    kind = _TYPES.get(t.dtype)
+    if kind is None or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
+    return kind
+
+
+def _hidden(H):
+    if H <= 0 or H % 128:
+        raise ValueError(f"columns must be a multiple of 128, got {H}")
+    return H
+
+
+def _order(order, device):
+    row0, row_pair, pair_row = order
+    for t, name, dim in ((row0, "expert_row0", 1), (row_pair, "row_pair", 1), (pair_row, "pair_row", 2)):
+        if t.dim() != dim:
+            raise ValueError(f"order.{name} must have {dim} dimension(s)")
+    if not 1 <= row0.numel() - 1 <= 512 or not 1 <= pair_row.shape[1] <= 8:
+        raise ValueError("an order has 1 to 512 local experts and 1 to 8 picks per token")
+    i32 = torch.int32
+    return (_in(row0, "order.expert_row0", device, i32), _in(row_pair, "order.row_pair", device, i32),
+            _in(pair_row, "order.pair_row", device, i32))
+
+
+def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0, align: int = 16,
+                max_rows: Optional[int] = None) -> TokenOrder:
+    """Expert-sorted tables of the picks `topk_idx` (int32 [T, top_k], as `MoELayer.route` gives them): every pick of an expert in
+    [local_expert_offset, local_expert_offset + num_local_experts) gets a row, in ascending (token, pick) order inside an expert, experts' segments
+    padded to multiples of `align` rows (a power of two up to 128).  Other picks get none.  `max_rows`: room of the row tensors, by default
+    enough for every case; pairs whose row would lie behind it get none."""
+    if topk_idx.dim() != 2 or topk_idx.dtype != torch.int32:
+        raise ValueError(f"topk_idx must be int32 [T, top_k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
+    device = _device(topk_idx, "topk_idx")
+    T, K = topk_idx.shape
+    El = int(num_local_experts)
+    if not 1 <= K <= 8 or not 1 <= El <= 512 or T * K > 1 << 30:
+        raise ValueError("1 to 8 picks per token, 1 to 512 local experts, at most 2^30 pairs")
+    if align not in (1, 2, 4, 8, 16, 32, 64, 128):
+        raise ValueError("align must be a power of two up to 128")
+    rows = T * K + (align - 1) * El if max_rows is None else int(max_rows)
+    if not 0 <= rows < 1 << 31 or not -(1 << 31) <= local_expert_offset < (1 << 31):
+        raise ValueError("max_rows or local_expert_offset out of range")
+    topk_idx = _in(topk_idx, "topk_idx", device, torch.int32)
+    n = C.c_size_t()
+    _lib.check(_lib.lib.b200moe_sort_workspace_bytes(T, K, El, C.byref(n)), "b200moe_sort_workspace_bytes")
+    dev = topk_idx.device
+    row0 = torch.empty(El + 1, dtype=torch.int32, device=dev)
+    row_pair = torch.empty(rows, dtype=torch.int32, device=dev)
+    pair_row = torch.empty(T, K, dtype=torch.int32, device=dev)
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+    _call("b200moe_sort_tokens", device, topk_idx.data_ptr(), T, K, El, local_expert_offset, align, rows, row0.data_ptr(),
+          row_pair.data_ptr(), pair_row.data_ptr(), None if ws is None else ws.data_ptr(), n.value)
+    return TokenOrder(row0, row_pair, pair_row)
+
+
+def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[T, H] -> [max_rows, H]: row r is the row of its pair's token, zeros in the padding of a segment."""
+    kind, device = _rows_type(x, "x"), _device(x, "x")
+    row0, row_pair, pair_row = _order(order, device)
+    T, K = pair_row.shape
+    H, R = _hidden(x.shape[1]), row_pair.numel()
+    x = _in(x, "x", device, x.dtype, (T, H), _ALIGN)
+    out = _out(out, "out", device, x.dtype, (R, H))
+    _apart(out, "out", x, row0, row_pair, pair_row)
+    _call("b200moe_permute", device, x.data_ptr(), kind, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T, K,
+          row0.numel() - 1, H, R, out.data_ptr())
+    return out
+
+
+def _combine(rows, w, order, out):
+    kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
+    row0, row_pair, pair_row = _order(order, device)
+    T, K = pair_row.shape
+    H, R = _hidden(rows.shape[1]), row_pair.numel()
+    rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
+    if w is not None:
+        w = _in(w, "topk_w", device, torch.float32, (T, K))
+    out = _out(out, "out", device, rows.dtype, (T, H))
+    _apart(out, "out", rows, pair_row, *(() if w is None else (w,)))
+    _call("b200moe_combine", device, rows.data_ptr(), kind, None if w is None else w.data_ptr(), pair_row.data_ptr(), T, K, H, R, out.data_ptr())
+    return out
+
+
+def permute_backward(grad_rows: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of `permute` (and of `restore_1x128`, as far as the activations go): [max_rows, H] -> [T, H], the sum over a
+    token's rows in fp32, rounded once."""
+    return _combine(grad_rows, None, order, out)
+
+
+def combine(rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[max_rows, H] and routing weights fp32 [T, top_k] -> [T, H]: the weighted sum over a token's rows in fp32, rounded once;
+    zeros for a token without rows."""
+    return _combine(rows, topk_w, order, out)
+
+
+def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None):
+    """Gradients of `combine`: (grad_rows [max_rows, H], grad_w fp32 [T, top_k]); `out` takes the first."""
+    kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
+    row0, row_pair, pair_row = _order(order, device)
+    T, K = pair_row.shape
+    H, R = _hidden(rows.shape[1]), row_pair.numel()
+    rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
+    grad_out = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
+    topk_w = _in(topk_w, "topk_w", device, torch.float32, (T, K))
+    out = _out(out, "out", device, rows.dtype, (R, H))
+    _apart(out, "out", rows, grad_out, topk_w, row0, row_pair, pair_row)
+    grad_w = torch.empty(T, K, dtype=torch.float32, device=rows.device)
+    _call("b200moe_combine_backward", device, grad_out.data_ptr(), rows.data_ptr(), kind, topk_w.data_ptr(), row0.data_ptr(),
+          row_pair.data_ptr(), pair_row.data_ptr(), T, K, row0.numel() - 1, H, R, out.data_ptr(), grad_w.data_ptr())
+    return out, grad_w
+
+
+def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrder] = None, dtype=torch.bfloat16,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Activations kept in 8 bits (e4m3 [T, H] and scales [H/128, T], as `quantize_1x128` makes them) read back as `dtype` (that of `out`, where it is
+    given): [T, H], or, with an order, rows in expert order like `permute`'s."""
+    if q.dim() != 2:
+        raise ValueError("q must be e4m3 [T, H]")
+    device = _device(q, "q")
+    T, H = q.shape[0], _hidden(q.shape[1])
+    if out is not None:
+        dtype = out.dtype
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"rows are bf16, fp16 or fp32, not {dtype}")
+    q = _in(q, "q", device, torch.float8_e4m3fn, None, 16)
+    scale = _in(scale, "scale", device, torch.float32, (H // 128, T))
+    if order is None:
+        out = _out(out, "out", device, dtype, (T, H))
+        _apart(out, "out", q, scale)
+        _call("b200moe_restore_1x128", device, q.data_ptr(), scale.data_ptr(), kind, None, None, None, T, 1, 1, H, T, out.data_ptr())
+        return out
+    row0, row_pair, pair_row = _order(order, device)
+    if pair_row.shape[0] != T:
+        raise ValueError(f"q has {T} tokens, the order {pair_row.shape[0]}")
+    R = row_pair.numel()
+    out = _out(out, "out", device, dtype, (R, H))
+    _apart(out, "out", q, scale, row0, row_pair, pair_row)
+    _call("b200moe_restore_1x128", device, q.data_ptr(), scale.data_ptr(), kind, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T,
+          pair_row.shape[1], row0.numel() - 1, H, R, out.data_ptr())
+    return out
+
+
+def _used(expert_row0, device):
+    """(the table kept alive, address of its last entry: the number of rows in use)"""
+    if expert_row0 is None:
+        return None, None
+    if expert_row0.dim() != 1 or expert_row0.numel() < 1:
+        raise ValueError("expert_row0 must be int32 [E_local + 1]")
+    t = _in(expert_row0, "expert_row0", device, torch.int32)
+    return t, t.data_ptr() + 4 * (t.numel() - 1)
+
+
+def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = None, out=None):
+    """[R, 2I] -> (act [R, I] = rows[:, :I] * silu(rows[:, I:]), q e4m3 [R, 2I], scale fp32 [2I/128, R]): the activation, and the 8-bit copy
+    of its inputs for `swiglu_backward`.  A group of 128 columns is scaled by the smallest power of two not below its largest
+    magnitude / 448; one that holds an infinity or a NaN gets the scale NaN.  `expert_row0`: only its last entry's number of rows is in use (None:
+    all).  `out`: the three tensors to write."""
+    kind, device = _rows_type(gemm1_rows, "gemm1_rows"), _device(gemm1_rows, "gemm1_rows")
+    R, I2 = gemm1_rows.shape
+    if I2 <= 0 or I2 % 256 or I2 > 1 << 21:
+        raise ValueError(f"gemm1_rows must have 2 * I columns, I a multiple of 128 up to 2^20, got {I2}")
+    keep, used = _used(expert_row0, device)
+    x = _in(gemm1_rows, "gemm1_rows", device, gemm1_rows.dtype, None, _ALIGN)
+    act, q, scale = (None, None, None) if out is None else out
+    act = _out(act, "act", device, x.dtype, (R, I2 // 2))
+    q = _out(q, "q", device, torch.float8_e4m3fn, (R, I2), 16)
+    scale = _out(scale, "scale", device, torch.float32, (I2 // 128, R), 4)
+    if out is not None:
+        _apart(act, "act", x, q, scale)
+        _apart(q, "q", x, scale)
+        _apart(scale, "scale", x)
+    _call("b200moe_swiglu_save", device, x.data_ptr(), kind, used, R, I2 // 2, act.data_ptr(), q.data_ptr(), scale.data_ptr())
+    return act, q, scale
+
+
+def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor, expert_row0: Optional[torch.Tensor] = None,
+                    with_act: bool = True, out=None):
+    """Gradient of `swiglu_save`'s activation from its 8-bit copy: (grad of gemm1_rows [R, 2I], act [R, I] again or None), both of
+    grad_act's type.  `out`: the two tensors to write (the second None without `with_act`)."""
+    kind, device = _rows_type(grad_act, "grad_act"), _device(grad_act, "grad_act")
+    R, I = grad_act.shape
+    if I <= 0 or I % 128 or I > 1 << 20:
+        raise ValueError(f"grad_act must have I columns, a multiple of 128 up to 2^20, got {I}")
+    keep, used = _used(expert_row0, device)
+    q = _in(q, "q", device, torch.float8_e4m3fn, (R, 2 * I), 16)
+    scale = _in(scale, "scale", device, torch.float32, (2 * I // 128, R))
+    grad_act = _in(grad_act, "grad_act", device, grad_act.dtype, None, _ALIGN)
+    grad_x, act = (None, None) if out is None else out
+    if act is not None and not with_act:
+        raise ValueError("out has a tensor for act, which with_act=False does not compute")
+    grad_x = _out(grad_x, "grad_gemm1_rows", device, grad_act.dtype, (R, 2 * I))
+    if with_act:
+        act = _out(act, "act", device, grad_act.dtype, (R, I))
+    if out is not None:
+        _apart(grad_x, "grad_gemm1_rows", q, scale, grad_act, *((act,) if with_act else ()))
+        if with_act:
+            _apart(act, "act", q, scale, grad_act)
+    _call("b200moe_swiglu_backward", device, q.data_ptr(), scale.data_ptr(), grad_act.data_ptr(), kind, used, R, I, grad_x.data_ptr(),
+          act.data_ptr() if with_act else None)
+    return grad_x, act
+
+
+def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Tensor], topk_idx: torch.Tensor, grad_w: torch.Tensor,
+                   routed_scaling_factor, routing_mode: int = ROUTING_DS, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the routing weights (`MoELayer.route` with the same logits, bias, factor and mode, which gave the picks
+    `topk_idx`) down to the logits: fp32 [T, E].  In modes 1 to 5 the bias's gradient is its column sum; in mode 0 the bias only selects."""
+    if routing_logits.dim() != 2 or topk_idx.dim() != 2:
+        raise ValueError("routing_logits must be [T, E] and topk_idx [T, top_k]")
+    device = _device(routing_logits, "routing_logits")
+    (T, E), K = routing_logits.shape, topk_idx.shape[1]
+    if E < 32 or E > 512 or E % 32 or not 1 <= K <= 8:
+        raise ValueError("E must be a multiple of 32 up to 512, top_k 1 to 8")
+    routing_mode = int(routing_mode)
+    if not 0 <= routing_mode <= 5 or (routing_mode == 4 and K != 1):
+        raise ValueError("routing_mode must be one of ROUTING_* (0 to 5; mode 4 picks one expert)")
+    logits = _in(routing_logits, "routing_logits", device, torch.float32, None, 16)
+    if routing_bias is not None:
+        routing_bias = _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,), 2)
+    topk_idx = _in(topk_idx, "topk_idx", device, torch.int32, (T, K))
+    grad_w = _in(grad_w, "grad_w", device, torch.float32, (T, K))
+    out = _out(out, "out", device, torch.float32, (T, E), 16)
+    _apart(out, "out", logits, topk_idx, grad_w, *(() if routing_bias is None else (routing_bias,)))
+    _call("b200moe_route_backward", device, logits.data_ptr(), None if routing_bias is None else routing_bias.data_ptr(), topk_idx.data_ptr(),
+          grad_w.data_ptr(), T, E, K, float(routed_scaling_factor), routing_mode, out.data_ptr())
+    return out
