@@ -81,139 +81,183 @@ __device__ __forceinline__ void store_elems(T* dst, const float* v) {
 }
 
 // ---------------------------------------------------------------- sort
-constexpr int SORT_THREADS = 1024;
-constexpr int SORT_SLICE = 2 * SORT_THREADS;      // pairs of a CTA where several share the work
-constexpr int SORT_ONE = 4 * SORT_THREADS;        // most pairs that one CTA sorts alone
+constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32;
+constexpr int SORT_ROUNDS = 4;                                 // pairs a thread holds
+constexpr int SORT_CHUNK = SORT_ROUNDS * SORT_THREADS;         // pairs of a CTA at a time
+constexpr int SORT_ALONE = 2 * SORT_THREADS;                   // most pairs that one CTA sorts alone
+static_assert(SORT_ALONE <= SORT_CHUNK, "one CTA holds all of its pairs");
 
 struct SortParams {
     const int32_t* topk_idx;      // [n], n = T K
     int n, num_local, local_offset, align, max_rows;
-    int* slices;                  // [CTAs][num_local] histogram per slice; several CTAs only
+    int slice;                    // pairs of a CTA, several CTAs only
+    int* slices;                  // [CTAs][sort_pitch(num_local)] histogram per slice; several CTAs only
     int32_t *expert_row0, *row_pair, *pair_row;
 };
 
-// First row of every expert from the counts, by one warp: lane l owns the experts [l per, (l + 1) per).
-__device__ __forceinline__ void sort_scan(const int* count, int num_local, int align, int* row0, int lane) {
-    const int per = (num_local + 31) / 32, e0 = lane * per;
-    int sum = 0;
-    for (int e = e0; e < min(e0 + per, num_local); ++e) sum += (count[e] + align - 1) & -align;
-    int upto = sum;
+__host__ __device__ constexpr int sort_pitch(int num_local) { return (num_local + 3) & ~3; }
+
+// Pairs of a thread in the chunk that starts at `begin`: as few as reach its end
+__device__ __forceinline__ int sort_rounds(int begin, int end) { return min((end - begin + SORT_THREADS - 1) / SORT_THREADS, SORT_ROUNDS); }
+
+// Ranks of up to SORT_CHUNK pairs from `begin` on: a warp takes 32 consecutive ones for each round and counts per expert in its
+// row of wcnt; a pair's rank among the warp's pairs of its expert is the count before its round + the lanes before it (match, popcount).
+__device__ __forceinline__ void sort_rank(const SortParams& p, int begin, int end, uint16_t (*wcnt)[ORDER_MAX_LOCAL + 2], int* le, int* rank) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rounds = sort_rounds(begin, end), first = begin + warp * (32 * rounds);
+#pragma unroll
+    for (int m = 0; m < SORT_ROUNDS; ++m) {
+        const int i = first + m * 32 + lane;
+        const bool on = m < rounds && i < end;
+        const int e = on ? __ldcg(p.topk_idx + i) : 0;
+        le[m] = on && e >= p.local_offset && (unsigned)e - (unsigned)p.local_offset < (unsigned)p.num_local ? e - p.local_offset : -1;
+        rank[m] = 0;
+    }
+    for (int e = lane; e < p.num_local; e += 32) wcnt[warp][e] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < SORT_ROUNDS; ++m) {
+        if (m >= rounds || first + m * 32 >= end) break;          // the same for the whole warp
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, le[m] >= 0 ? le[m] : -1 - lane);
+        const int before = le[m] >= 0 ? wcnt[warp][le[m]] : 0, in = __popc(same & ((1u << lane) - 1u));
+        rank[m] = before + in;
+        __syncwarp();
+        if (le[m] >= 0 && in == 0) wcnt[warp][le[m]] = (uint16_t)(before + __popc(same));
+        __syncwarp();
+    }
+}
+
+// Exclusive prefix over the warps of an expert's counts (thread e: expert e); returns the expert's number of pairs
+__device__ __forceinline__ int sort_over_warps(uint16_t (*wcnt)[ORDER_MAX_LOCAL + 2], int e) {
+    int r = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) { const int v = wcnt[w][e]; wcnt[w][e] = (uint16_t)r; r += v; }
+    return r;
+}
+
+// Exclusive prefix of the padded counts (thread e < ORDER_MAX_LOCAL: expert e's, 0 behind the last), for all threads of the CTA, which meet here
+__device__ __forceinline__ int sort_rows_before(int count, int align, int* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int padded = (count + align - 1) & -align;
+    int upto = padded;
+#pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(0xFFFFFFFFu, upto, off);
         if (lane >= off) upto += v;
     }
-    int r = upto - sum;
-    for (int e = e0; e < min(e0 + per, num_local); ++e) { row0[e] = r; r += (count[e] + align - 1) & -align; }
-    if (lane == 31) row0[num_local] = upto;
+    if (lane == 31) s_warp[warp] = upto;
+    __syncthreads();
+    int r = upto - padded;
+#pragma unroll
+    for (int w = 0; w < ORDER_MAX_LOCAL / 32; ++w) r += w < warp ? s_warp[w] : 0;
+    return r;
 }
 
-// Places the pairs [begin, end), 1024 at a time: next[e] = row of the expert's next pair, moved on by the pairs placed.
-// A pair's rank among the pairs of its expert: match + popcount inside its warp, a prefix over the 32 warps.
-__device__ __forceinline__ void sort_place(const SortParams& p, int begin, int end, int* next, uint16_t (*wcnt)[ORDER_MAX_LOCAL + 2]) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, El = p.num_local;
-    const unsigned FULL = 0xFFFFFFFFu;
-    for (int c = begin; c < end; c += SORT_THREADS) {
-        for (int e = lane; e < El; e += 32) wcnt[warp][e] = 0;
-        __syncwarp();
-        const int i = c + tid;
-        const int le = i < end ? __ldg(p.topk_idx + i) - p.local_offset : -1;
-        const bool local = le >= 0 && le < El;
-        const unsigned same = __match_any_sync(FULL, local ? le : -1 - lane);
-        const int rank = __popc(same & ((1u << lane) - 1u));
-        if (local && rank == 0) wcnt[warp][le] = (uint16_t)__popc(same);
-        __syncthreads();
-        for (int e = tid; e < El; e += SORT_THREADS) {
-            int r = 0;
-#pragma unroll 8
-            for (int w = 0; w < 32; ++w) { const int v = wcnt[w][e]; wcnt[w][e] = (uint16_t)r; r += v; }
-            wcnt[32][e] = (uint16_t)r;
-        }
-        __syncthreads();
-        if (i < end) {
-            int r = local ? next[le] + wcnt[warp][le] + rank : -1;
+// Rows of the pairs that sort_rank saw: next[e] = row of the expert's first pair among them
+__device__ __forceinline__ void sort_store(const SortParams& p, int begin, int end, const int* next, uint16_t (*wcnt)[ORDER_MAX_LOCAL + 2], const int* le,
+                                           const int* rank) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rounds = sort_rounds(begin, end);
+#pragma unroll
+    for (int m = 0; m < SORT_ROUNDS; ++m) {
+        const int i = begin + (warp * rounds + m) * 32 + lane;
+        if (m < rounds && i < end) {
+            int r = le[m] >= 0 ? next[le[m]] + wcnt[warp][le[m]] + rank[m] : -1;
             if (r >= p.max_rows) r = -1;
             p.pair_row[i] = r;
             if (r >= 0) p.row_pair[r] = i;
         }
-        __syncthreads();
-        for (int e = tid; e < El; e += SORT_THREADS) next[e] += wcnt[32][e];
     }
 }
 
-// One CTA for everything: counts, scan, places.
+// One CTA for up to SORT_ALONE pairs
 __global__ void __launch_bounds__(SORT_THREADS) sort_one_kernel(const SortParams p) {
-    __shared__ int s_count[ORDER_MAX_LOCAL], s_next[ORDER_MAX_LOCAL + 1];
-    __shared__ uint16_t s_wcnt[33][ORDER_MAX_LOCAL + 2];
+    __shared__ int s_next[ORDER_MAX_LOCAL], s_warp[SORT_WARPS];
+    __shared__ uint16_t s_wcnt[SORT_WARPS][ORDER_MAX_LOCAL + 2];
     const int tid = threadIdx.x;
-    for (int e = tid; e < p.num_local; e += SORT_THREADS) s_count[e] = 0;
     pdl_wait();
     pdl_launch();
-    __syncthreads();
-    for (int i = tid; i < p.n; i += SORT_THREADS) {
-        const int le = __ldg(p.topk_idx + i) - p.local_offset;
-        if (le >= 0 && le < p.num_local) atomicAdd(s_count + le, 1);
-    }
+    int le[SORT_ROUNDS], rank[SORT_ROUNDS];
+    sort_rank(p, 0, p.n, s_wcnt, le, rank);
     for (int r = tid; r < p.max_rows; r += SORT_THREADS) p.row_pair[r] = -1;
     __syncthreads();
-    if (tid < 32) sort_scan(s_count, p.num_local, p.align, s_next, tid);
+    const int count = tid < p.num_local ? sort_over_warps(s_wcnt, tid) : 0;
+    const int r0 = sort_rows_before(count, p.align, s_warp);
+    if (tid < p.num_local) s_next[tid] = r0;
+    if (tid <= p.num_local) p.expert_row0[tid] = min(r0, p.max_rows);
     __syncthreads();
-    for (int e = tid; e <= p.num_local; e += SORT_THREADS) p.expert_row0[e] = min(s_next[e], p.max_rows);
-    __syncthreads();
-    sort_place(p, 0, p.n, s_next, s_wcnt);
+    sort_store(p, 0, p.n, s_next, s_wcnt, le, rank);
 }
 
 // Several CTAs, first kernel: the slice's histogram; row_pair is cleared for the second one.
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortParams p) {
     __shared__ int s_count[ORDER_MAX_LOCAL];
     const int tid = threadIdx.x;
-    for (int e = tid; e < p.num_local; e += SORT_THREADS) s_count[e] = 0;
+    const int pitch = sort_pitch(p.num_local);
+    if (tid < pitch) s_count[tid] = 0;
     pdl_wait();
     pdl_launch();
     __syncthreads();
-    const int begin = blockIdx.x * SORT_SLICE, end = min(p.n, begin + SORT_SLICE);
-    for (int i = begin + tid; i < end; i += SORT_THREADS) {
-        const int le = __ldg(p.topk_idx + i) - p.local_offset;
-        if (le >= 0 && le < p.num_local) atomicAdd(s_count + le, 1);
+    const long long begin = (long long)blockIdx.x * p.slice;
+    const int end = (int)min((long long)p.n, begin + p.slice);
+    for (long long i = begin + tid; i < end; i += SORT_THREADS) {
+        const int e = __ldg(p.topk_idx + i);
+        if (e >= p.local_offset && (unsigned)e - (unsigned)p.local_offset < (unsigned)p.num_local) atomicAdd(s_count + (e - p.local_offset), 1);
     }
-    for (int r = blockIdx.x * SORT_THREADS + tid; r < p.max_rows; r += gridDim.x * SORT_THREADS) p.row_pair[r] = -1;
+    for (long long r = blockIdx.x * (long long)SORT_THREADS + tid; r < p.max_rows; r += gridDim.x * (long long)SORT_THREADS) p.row_pair[r] = -1;
     __syncthreads();
-    for (int e = tid; e < p.num_local; e += SORT_THREADS) p.slices[(size_t)blockIdx.x * p.num_local + e] = s_count[e];
+    if (tid < pitch) p.slices[(size_t)blockIdx.x * pitch + tid] = s_count[tid];
 }
 
 // Second kernel: every CTA sums the histograms (all of them: the first rows; those before its own: where its pairs start
 // inside a segment) and places its slice.  No CTA waits for another.
 __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortParams p) {
-    __shared__ int s_count[ORDER_MAX_LOCAL], s_before[ORDER_MAX_LOCAL], s_next[ORDER_MAX_LOCAL + 1];
-    __shared__ uint16_t s_wcnt[33][ORDER_MAX_LOCAL + 2];
+    __shared__ int s_count[ORDER_MAX_LOCAL], s_next[ORDER_MAX_LOCAL], s_warp[SORT_WARPS];
+    __shared__ uint16_t s_wcnt[SORT_WARPS][ORDER_MAX_LOCAL + 2];
     const int tid = threadIdx.x, El = p.num_local, c = blockIdx.x;
-    for (int e = tid; e < El; e += SORT_THREADS) { s_count[e] = 0; s_before[e] = 0; }
+    if (tid < ORDER_MAX_LOCAL) { s_count[tid] = 0; s_next[tid] = 0; }
+    const int begin = (int)((long long)c * p.slice), end = (int)min((long long)p.n, (long long)begin + p.slice);
+    int le[SORT_ROUNDS], rank[SORT_ROUNDS];
+    // The ids were there before any CTA of the first kernel let this one start; they are read past L1.
+    sort_rank(p, begin, end, s_wcnt, le, rank);
+    __syncthreads();
     pdl_wait();
     pdl_launch();
-    __syncthreads();
-    int width = 32;                                   // threads of one row of the table
-    while (width < El) width <<= 1;
-    const int e = tid & (width - 1);
-    if (e < El) {
-        int total = 0, before = 0;
-#pragma unroll 4
+    // four experts per load, eight rows of the table in flight (111 slices of 256 experts: 8 us with one expert per load)
+    const int quads = sort_pitch(El) >> 2;
+    int width = 8;                                    // threads of one row of the table
+    while (width < quads) width <<= 1;
+    const int e4 = tid & (width - 1);
+    if (e4 < quads) {
+        int total[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0};
+#pragma unroll 8
         for (int s = tid / width; s < (int)gridDim.x; s += SORT_THREADS / width) {
-            const int v = p.slices[(size_t)s * El + e];
-            total += v;
-            if (s < c) before += v;
+            const int4 v = __ldcg(reinterpret_cast<const int4*>(p.slices) + (size_t)s * quads + e4);
+            const int first = s < c;
+            total[0] += v.x; total[1] += v.y; total[2] += v.z; total[3] += v.w;
+            before[0] += first * v.x; before[1] += first * v.y; before[2] += first * v.z; before[3] += first * v.w;
         }
-        atomicAdd(s_count + e, total);
-        atomicAdd(s_before + e, before);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (total[i]) atomicAdd(s_count + 4 * e4 + i, total[i]);
+            if (before[i]) atomicAdd(s_next + 4 * e4 + i, before[i]);
+        }
     }
+    int here = tid < El ? sort_over_warps(s_wcnt, tid) : 0;
     __syncthreads();
-    if (tid < 32) sort_scan(s_count, El, p.align, s_next, tid);
+    const int r0 = sort_rows_before(tid < El ? s_count[tid] : 0, p.align, s_warp);
+    if (tid < El) s_next[tid] += r0;
+    if (c == 0 && tid <= El) p.expert_row0[tid] = min(r0, p.max_rows);
     __syncthreads();
-    if (c == 0)
-        for (int k = tid; k <= El; k += SORT_THREADS) p.expert_row0[k] = min(s_next[k], p.max_rows);
-    __syncthreads();
-    for (int k = tid; k < El; k += SORT_THREADS) s_next[k] += s_before[k];
-    __syncthreads();
-    const int begin = c * SORT_SLICE;
-    sort_place(p, begin, min(p.n, begin + SORT_SLICE), s_next, s_wcnt);
+    sort_store(p, begin, end, s_next, s_wcnt, le, rank);
+    for (int at = begin + SORT_CHUNK; at < end; at += SORT_CHUNK) {      // (a slice is no longer than 2^30, so `at` stays below 2^31)
+        __syncthreads();
+        if (tid < El) s_next[tid] += here;
+        sort_rank(p, at, end, s_wcnt, le, rank);
+        __syncthreads();
+        here = tid < El ? sort_over_warps(s_wcnt, tid) : 0;
+        __syncthreads();
+        sort_store(p, at, end, s_next, s_wcnt, le, rank);
+    }
 }
 
 // ---------------------------------------------------------------- rows into expert order
@@ -224,54 +268,69 @@ struct OrderParams {
     int T, top_k, num_local, num_rows;
 };
 
-// Zeros into the padding rows of the segments, `units` of 32 bytes each: a warp looks at 32 rows at a time.
-__device__ __forceinline__ void zero_padding(const OrderParams& o, char* rows, int units, int warp, int warps) {
-    const int lane = threadIdx.x & 31;
-    const int used = min(__ldg(o.expert_row0 + o.num_local), o.num_rows);
-    for (int r0 = warp * 32; r0 < used; r0 += warps * 32) {
-        const int pair = r0 + lane < used ? __ldg(o.row_pair + r0 + lane) : 0;
-        unsigned empty = __ballot_sync(0xFFFFFFFFu, pair < 0);
-        while (empty) {
-            const int r = r0 + __ffs(empty) - 1;
-            empty &= empty - 1;
-            char* dst = rows + (size_t)r * units * 32;
-            for (int u = lane; u < units; u += 32) st_global_v8(dst + (size_t)u * 32, 0, 0, 0, 0, 0, 0, 0, 0);
-        }
+// The row kernels below deal 32-byte units (16 columns of 16 bits, 8 of 32) of all tokens' rows out to consecutive threads, so that
+// no width leaves lanes idle: unit g belongs to token g / units.
+struct Unit { int token, unit; };
+__device__ __forceinline__ Unit unit_of(unsigned long long g, unsigned units) {
+    const unsigned t = g >> 32 ? (unsigned)(g / units) : (unsigned)g / units;
+    return {(int)t, (int)(g - (unsigned long long)t * units)};
+}
+
+// Rows of token t, -1 where a pick has none
+__device__ __forceinline__ void token_rows(const OrderParams& o, int t, int* r) {
+#pragma unroll
+    for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
+        r[k] = k < o.top_k ? __ldg(o.pair_row + (size_t)t * o.top_k + k) : -1;
+        if (r[k] >= o.num_rows) r[k] = -1;
     }
 }
 
-// rows[r] = x[t] for the token's rows: a warp takes a token (and one of gridDim.y parts of its columns), reads each 32
-// bytes once and stores them up to top_k times.
-constexpr int PERMUTE_FLIGHT = 4;
-__global__ void __launch_bounds__(256) permute_rows_kernel(const OrderParams o, const char* __restrict__ x, char* __restrict__ rows, int units) {
-    const int lane = threadIdx.x & 31;
-    const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, warps = (gridDim.x * blockDim.x) >> 5;
-    const int per = (units + gridDim.y - 1) / gridDim.y, u_lo = blockIdx.y * per, u_hi = min(units, u_lo + per);
-    pdl_wait();
-    for (int t = warp; t < o.T; t += warps) {
-        int r = -1;
-        if (lane < o.top_k) {
-            r = __ldg(o.pair_row + (size_t)t * o.top_k + lane);
-            if (r >= o.num_rows) r = -1;
-        }
-        const unsigned have = __ballot_sync(0xFFFFFFFFu, r >= 0);
-        const char* src = x + (size_t)t * units * 32;
-        for (int u0 = u_lo + lane; u0 - lane < u_hi; u0 += 32 * PERMUTE_FLIGHT) {
-            uint32_t v[PERMUTE_FLIGHT][8];
-#pragma unroll
-            for (int q = 0; q < PERMUTE_FLIGHT; ++q)
-                if (have && u0 + 32 * q < u_hi) ld_global_v8(src + (size_t)(u0 + 32 * q) * 32, v[q]);
-            for (unsigned todo = have; todo; todo &= todo - 1) {
-                char* dst = rows + (size_t)__shfl_sync(0xFFFFFFFFu, r, __ffs(todo) - 1) * units * 32;
-#pragma unroll
-                for (int q = 0; q < PERMUTE_FLIGHT; ++q)
-                    if (u0 + 32 * q < u_hi)
-                        st_global_v8(dst + (size_t)(u0 + 32 * q) * 32, v[q][0], v[q][1], v[q][2], v[q][3], v[q][4], v[q][5], v[q][6], v[q][7]);
+// Zeros into the padding rows of the segments.  Every warp owns a block of up to 32 consecutive rows (several where there are more rows than
+// that).  Which rows of the first block are padding is looked up early (begin) and acted on behind the kernel's own work, so that
+// the look-up's latency hides.
+struct Padding {
+    int used, pair;
+    static __device__ __forceinline__ int warp() { return (int)((blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x) >> 5); }
+    static __device__ __forceinline__ int warps() { return (int)((gridDim.x * (unsigned long long)blockDim.x) >> 5); }
+    static __device__ __forceinline__ int per(const OrderParams& o) { return min(32, (o.num_rows - 1) / warps() + 1); }
+    __device__ __forceinline__ void begin(const OrderParams& o) {
+        used = min(__ldg(o.expert_row0 + o.num_local), o.num_rows);
+        const int lane = threadIdx.x & 31, n = per(o);
+        const long long r = (long long)warp() * n + lane;
+        pair = lane < n && r < used ? __ldg(o.row_pair + r) : 0;
+    }
+    __device__ __forceinline__ void fill(const OrderParams& o, char* rows, int units) {
+        const int lane = threadIdx.x & 31, n = per(o);
+        for (long long r0 = (long long)warp() * n;;) {
+            for (unsigned empty = __ballot_sync(0xFFFFFFFFu, pair < 0); empty; empty &= empty - 1) {
+                char* dst = rows + (size_t)(r0 + __ffs(empty) - 1) * units * 32;
+                for (int u = lane; u < units; u += 32) st_global_v8(dst + (size_t)u * 32, 0, 0, 0, 0, 0, 0, 0, 0);
             }
+            r0 += (long long)warps() * n;
+            if (r0 >= used) break;
+            pair = lane < n && r0 + lane < used ? __ldg(o.row_pair + r0 + lane) : 0;
         }
     }
+};
+
+// rows[r] = x[t] for the token's rows: a unit is read once and stored up to top_k times.
+__global__ void __launch_bounds__(256) permute_rows_kernel(const OrderParams o, const char* __restrict__ x, char* __restrict__ rows, int units) {
+    pdl_wait();
+    Padding pad;
+    pad.begin(o);
+    const unsigned long long total = (unsigned long long)o.T * units, step = (unsigned long long)gridDim.x * blockDim.x;
+    for (unsigned long long g = blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x; g < total; g += step) {
+        const Unit at = unit_of(g, units);
+        uint32_t v[8];
+        ld_global_v8(x + g * 32, v);
+        int r[ORDER_MAX_PICKS];
+        token_rows(o, at.token, r);
+#pragma unroll
+        for (int k = 0; k < ORDER_MAX_PICKS; ++k)
+            if (r[k] >= 0) st_global_v8(rows + ((size_t)r[k] * units + at.unit) * 32, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+    }
     pdl_launch();
-    if (blockIdx.y == 0) zero_padding(o, rows, units, warp, warps);
+    pad.fill(o, rows, units);
 }
 
 // 16 e4m3 values times their scale
@@ -284,157 +343,270 @@ __device__ __forceinline__ void restore16(const uint4& q, float s, float* v) {
     }
 }
 
-// rows[r] = q[t] * scale, like permute_rows_kernel with 16 columns per lane and step.  Without an order (pair_row null)
-// row t is token t.
+// rows[r] = q[t] * scale, like permute_rows_kernel with units of 16 columns.  Without an order (pair_row null) row t is token t.
 template <typename T>
 __global__ void __launch_bounds__(256) restore_rows_kernel(const OrderParams o, const uint8_t* __restrict__ q, const float* __restrict__ scale,
                                                            T* __restrict__ rows, int H) {
-    const int lane = threadIdx.x & 31;
-    const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, warps = (gridDim.x * blockDim.x) >> 5;
-    const int units = H >> 4;
-    const int per = (units + gridDim.y - 1) / gridDim.y, u_lo = blockIdx.y * per, u_hi = min(units, u_lo + per);
     pdl_wait();
-    for (int t = warp; t < o.T; t += warps) {
-        int r = -1;
-        if (!o.pair_row) {
-            if (lane == 0) r = t;
-        } else if (lane < o.top_k) {
-            r = __ldg(o.pair_row + (size_t)t * o.top_k + lane);
-            if (r >= o.num_rows) r = -1;
+    const bool ordered = o.pair_row != nullptr;
+    const int units = H >> 4;
+    Padding pad;
+    if (ordered) pad.begin(o);
+    const unsigned long long total = (unsigned long long)o.T * units, step = (unsigned long long)gridDim.x * blockDim.x;
+    for (unsigned long long g = blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x; g < total; g += step) {
+        const Unit at = unit_of(g, units);
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(q) + g);
+        const float s = __ldg(scale + (size_t)(at.unit >> 3) * o.T + at.token);
+        float v[16];
+        if (!ordered) {
+            restore16(b, s, v);
+            store_elems<T, 16>(rows + g * 16, v);
+            continue;
         }
-        const unsigned have = __ballot_sync(0xFFFFFFFFu, r >= 0);
-        if (!have) continue;
-        for (int u0 = u_lo; u0 < u_hi; u0 += 32) {
-            const int u = u0 + lane;
-            float v[16];
-            if (u < u_hi) {
-                const uint4 b = __ldg(reinterpret_cast<const uint4*>(q + (size_t)t * H) + u);
-                restore16(b, __ldg(scale + (size_t)(u >> 3) * o.T + t), v);
-            }
-            for (unsigned todo = have; todo; todo &= todo - 1) {
-                T* dst = rows + (size_t)__shfl_sync(0xFFFFFFFFu, r, __ffs(todo) - 1) * H;
-                if (u < u_hi) store_elems<T, 16>(dst + u * 16, v);
-            }
-        }
+        int r[ORDER_MAX_PICKS];
+        token_rows(o, at.token, r);
+        restore16(b, s, v);
+#pragma unroll
+        for (int k = 0; k < ORDER_MAX_PICKS; ++k)
+            if (r[k] >= 0) store_elems<T, 16>(rows + (size_t)r[k] * H + at.unit * 16, v);
     }
     pdl_launch();
-    if (o.pair_row && blockIdx.y == 0) zero_padding(o, reinterpret_cast<char*>(rows), H * (int)sizeof(T) / 32, warp, warps);
+    if (ordered) pad.fill(o, reinterpret_cast<char*>(rows), H * (int)sizeof(T) / 32);
 }
 
 // ---------------------------------------------------------------- rows back to their tokens
-// out[t] = sum_k w[t, k] rows[r(t, k)], w null: ones.  A warp takes a token (and one of gridDim.y parts of its columns); the
-// loads of up to eight rows are in flight together.
-template <typename T>
-__global__ void __launch_bounds__(256) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
-                                                           T* __restrict__ out, int H) {
-    constexpr int V = 16 / sizeof(T);
-    const int lane = threadIdx.x & 31;
-    const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, warps = (gridDim.x * blockDim.x) >> 5;
-    const int units = H / V;
-    const int per = (units + gridDim.y - 1) / gridDim.y, u_lo = blockIdx.y * per, u_hi = min(units, u_lo + per);
+// out[t] = sum_k w[t, k] rows[r(t, k)], w null: ones.  A thread takes 32-byte units, one after the other: while the rows of one are on their
+// way it looks up the rows of the next, so that the chain of dependent loads is paid once.  FLIGHT rows' loads are in flight together.
+template <typename T, int FLIGHT, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
+                                                                     T* __restrict__ out, int H) {
+    constexpr int V = 32 / sizeof(T), K = ORDER_MAX_PICKS;
     pdl_wait();
-    for (int t = warp; t < o.T; t += warps) {
-        int r = -1;
-        float wt = 1.f;
-        if (lane < o.top_k) {
-            r = __ldg(o.pair_row + (size_t)t * o.top_k + lane);
-            if (r >= o.num_rows) r = -1;
-            if (w) wt = __ldg(w + (size_t)t * o.top_k + lane);
-        }
-        for (int u0 = u_lo; u0 < u_hi; u0 += 32) {
-            const int u = u0 + lane;
-            uint4 v[ORDER_MAX_PICKS];
-#pragma unroll
-            for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
-                const int rk = __shfl_sync(0xFFFFFFFFu, r, k);
-                if (rk >= 0 && u < u_hi) v[k] = __ldcs(reinterpret_cast<const uint4*>(rows + (size_t)rk * H) + u);
-            }
+    const int units = H / V;
+    const unsigned long long total = (unsigned long long)o.T * units, step = (unsigned long long)gridDim.x * blockDim.x;
+    unsigned long long g = blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x;
+    if (g < total) {
+        Unit at = unit_of(g, units);
+        int r[K];
+        token_rows(o, at.token, r);
+        while (true) {
+            const unsigned long long next = g + step;
+            Unit at2 = {0, 0};
+            int r2[K];
             float acc[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
-                const int rk = __shfl_sync(0xFFFFFFFFu, r, k);
-                const float wk = __shfl_sync(0xFFFFFFFFu, wt, k);
-                if (rk >= 0 && u < u_hi) {
-                    const uint32_t b[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            for (int k0 = 0; k0 < K; k0 += FLIGHT) {
+                uint32_t v[FLIGHT][8];
+                float wk[FLIGHT];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (sizeof(T) == 4) {
-                            acc[i] = fmaf(wk, __uint_as_float(b[i]), acc[i]);
-                        } else {
-                            const float2 f = Elem<T>::unpack(b[i]);
-                            acc[2 * i] = fmaf(wk, f.x, acc[2 * i]); acc[2 * i + 1] = fmaf(wk, f.y, acc[2 * i + 1]);
-                        }
+                for (int k = 0; k < FLIGHT; ++k)
+                    if (r[k0 + k] >= 0) {
+                        ld_global_v8(rows + (size_t)r[k0 + k] * H + at.unit * V, v[k]);
+                        wk[k] = w ? __ldg(w + (size_t)at.token * o.top_k + k0 + k) : 1.f;
                     }
+                if (k0 + FLIGHT == K && next < total) {
+                    at2 = unit_of(next, units);
+                    token_rows(o, at2.token, r2);
                 }
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k)
+                    if (r[k0 + k] >= 0)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if constexpr (sizeof(T) == 4) {
+                                acc[i] = fmaf(wk[k], __uint_as_float(v[k][i]), acc[i]);
+                            } else {
+                                const float2 f = Elem<T>::unpack(v[k][i]);
+                                acc[2 * i] = fmaf(wk[k], f.x, acc[2 * i]); acc[2 * i + 1] = fmaf(wk[k], f.y, acc[2 * i + 1]);
+                            }
+                        }
             }
-            if (u < u_hi) store_elems<T, V>(out + (size_t)t * H + u * V, acc);
+            store_elems<T, V>(out + g * V, acc);
+            if (next >= total) break;
+            g = next; at = at2;
+#pragma unroll
+            for (int k = 0; k < K; ++k) r[k] = r2[k];
         }
     }
     pdl_launch();
 }
 
-// d_rows[r] = w d_out[t] and d_w[t, k] = <d_out[t], rows[r]>: a CTA takes a token, so that the products' sums stay inside it.
+// Sums of eight values over the 32 lanes in nine shuffles instead of forty: three steps halve what a lane carries, two more add.  Lane l
+// returns the sum of value l >> 2.
+__device__ __forceinline__ float warp_sums8(const float* v, int lane) {
+    float a[4], b[2], c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float keep = lane & 16 ? v[i + 4] : v[i], give = lane & 16 ? v[i] : v[i + 4];
+        a[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float keep = lane & 8 ? a[i + 2] : a[i], give = lane & 8 ? a[i] : a[i + 2];
+        b[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, 8);
+    }
+    {
+        const float keep = lane & 4 ? b[1] : b[0], give = lane & 4 ? b[0] : b[1];
+        c = keep + __shfl_xor_sync(0xFFFFFFFFu, give, 4);
+    }
+    c += __shfl_xor_sync(0xFFFFFFFFu, c, 2);
+    return c + __shfl_xor_sync(0xFFFFFFFFu, c, 1);
+}
+
+// 16 bytes of a row as fp32 values
 template <typename T>
-__global__ void __launch_bounds__(256) combine_grad_kernel(const OrderParams o, const T* __restrict__ d_out, const T* __restrict__ rows,
-                                                           const float* __restrict__ w, T* __restrict__ d_rows, float* __restrict__ d_w, int H) {
-    constexpr int V = 16 / sizeof(T);
-    __shared__ float s_dot[2][8][ORDER_MAX_PICKS];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    const int units = H / V;
-    pdl_wait();
-    int buf = 0;
-    for (int t = blockIdx.x; t < o.T; t += gridDim.x, buf ^= 1) {
-        int rk[ORDER_MAX_PICKS];
-        float wk[ORDER_MAX_PICKS], dot[ORDER_MAX_PICKS];
+__device__ __forceinline__ void unpack16(const uint4& q, float* v) {
+    const uint32_t b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
-            rk[k] = k < o.top_k ? __ldg(o.pair_row + (size_t)t * o.top_k + k) : -1;
-            if (rk[k] >= o.num_rows) rk[k] = -1;
-            wk[k] = k < o.top_k ? __ldg(w + (size_t)t * o.top_k + k) : 0.f;
-            dot[k] = 0.f;
-        }
-        for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            float g[V];
-            load_elems<T, V>(d_out + (size_t)t * H + u * V, g);
-            uint4 v[ORDER_MAX_PICKS];
-#pragma unroll
-            for (int k = 0; k < ORDER_MAX_PICKS; ++k)
-                if (rk[k] >= 0) v[k] = __ldcs(reinterpret_cast<const uint4*>(rows + (size_t)rk[k] * H) + u);
-#pragma unroll
-            for (int k = 0; k < ORDER_MAX_PICKS; ++k)
-                if (rk[k] >= 0) {
-                    const uint32_t b[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-                    float y[V];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (sizeof(T) == 4) {
-                            dot[k] = fmaf(g[i], __uint_as_float(b[i]), dot[k]);
-                        } else {
-                            const float2 f = Elem<T>::unpack(b[i]);
-                            dot[k] = fmaf(g[2 * i], f.x, dot[k]); dot[k] = fmaf(g[2 * i + 1], f.y, dot[k]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) y[i] = wk[k] * g[i];
-                    store_elems<T, V>(d_rows + (size_t)rk[k] * H + u * V, y);
-                }
-        }
-#pragma unroll
-        for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
-            for (int off = 16; off; off >>= 1) dot[k] += __shfl_xor_sync(0xFFFFFFFFu, dot[k], off);
-            if (lane == 0) s_dot[buf][wid][k] = dot[k];
-        }
-        __syncthreads();      // (two buffers: a warp is at most one token ahead of the thread that sums)
-        if (threadIdx.x < o.top_k) {
-            float sum = 0.f;
-            for (int i = 0; i < nw; ++i) sum += s_dot[buf][i][threadIdx.x];
-            d_w[(size_t)t * o.top_k + threadIdx.x] = sum;
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(b[i]);
+        } else {
+            const float2 f = Elem<T>::unpack(b[i]);
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
         }
     }
-    pdl_launch();
-    zero_padding(o, reinterpret_cast<char*>(d_rows), H * (int)sizeof(T) / 32, blockIdx.x * nw + wid, gridDim.x * nw);
+}
+
+// One unit of one row: its part of the product's sum, and w times the gradient stored
+template <typename T>
+__device__ __forceinline__ float grad_unit(const float* g, const uint4& row, float w, T* dst, float dot) {
+    constexpr int V = 16 / sizeof(T);
+    float y[V];
+    unpack16<T>(row, y);
+#pragma unroll
+    for (int i = 0; i < V; ++i) { dot = fmaf(g[i], y[i], dot); y[i] = w * g[i]; }
+    store_elems<T, V>(dst, y);
+    return dot;
+}
+
+// d_rows[r] = w d_out[t] and d_w[t, k] = <d_out[t], rows[r]>, two ways.
+// By tokens: a group of threads (whole warps) takes a token with all of its rows, so that d_out is read once and eight rows' loads are in
+// flight.  By rows: a group takes a row, with FLIGHT units of it in flight per thread, whichever token it belongs to; d_out comes from L2
+// as often as it has rows.
+constexpr int GRAD_FLIGHT = 4;
+template <typename T>
+__device__ __forceinline__ void combine_grad_by_rows(const OrderParams& o, const T* __restrict__ d_out, const T* __restrict__ rows, const float* __restrict__ w,
+                                                     T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, int used, float (*s_dot)[8][ORDER_MAX_PICKS]) {
+    constexpr int V = 16 / sizeof(T), FLIGHT = GRAD_FLIGHT;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int groups = 256 >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
+    const int units = H / V, pairs = o.T * o.top_k;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pairs; i += gridDim.x * 256ll) {
+        const int r = __ldg(o.pair_row + i);
+        if (r < 0 || r >= o.num_rows) d_w[i] = 0.f;
+    }
+    int buf = 0;
+    for (long long r0 = (long long)blockIdx.x * groups; r0 < used; r0 += (long long)gridDim.x * groups, buf ^= 1) {
+        const long long r = r0 + (threadIdx.x >> gsh);
+        int pair = -1;
+        float dot = 0.f;
+        if (r < used) {
+            pair = __ldg(o.row_pair + r);
+            if (pair >= pairs) pair = -1;
+            T* dst = d_rows + (size_t)r * H;
+            if (pair < 0) {
+                for (int u = in; u < units / 2; u += stride) st_global_v8(reinterpret_cast<char*>(dst) + (size_t)u * 32, 0, 0, 0, 0, 0, 0, 0, 0);
+            } else {
+                const float wk = __ldg(w + pair);
+                const uint4 *src = reinterpret_cast<const uint4*>(d_out + (size_t)(pair / o.top_k) * H),
+                            *row = reinterpret_cast<const uint4*>(rows + (size_t)r * H);
+                for (int u0 = in; u0 < units; u0 += FLIGHT * stride) {
+                    uint4 d[FLIGHT], v[FLIGHT];
+#pragma unroll
+                    for (int q = 0; q < FLIGHT; ++q)
+                        if (u0 + q * stride < units) { d[q] = __ldg(src + u0 + q * stride); v[q] = __ldcs(row + u0 + q * stride); }
+#pragma unroll
+                    for (int q = 0; q < FLIGHT; ++q)
+                        if (u0 + q * stride < units) {
+                            float g[V];
+                            unpack16<T>(d[q], g);
+                            dot = grad_unit<T>(g, v[q], wk, dst + (u0 + q * stride) * V, dot);
+                        }
+                }
+            }
+        }
+        for (int off = 16; off; off >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, off);
+        if (gsh > 5) {
+            if (lane == 0) s_dot[buf][wid][0] = dot;
+            __syncthreads();
+            if (in == 0) {
+                dot = 0.f;
+                for (int i = 0; i < stride >> 5; ++i) dot += s_dot[buf][wid + i][0];
+            }
+        }
+        if (in == 0 && pair >= 0) d_w[pair] = dot;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void combine_grad_by_tokens(const OrderParams& o, const T* __restrict__ d_out, const T* __restrict__ rows, const float* __restrict__ w,
+                                                       T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, float (*s_dot)[8][ORDER_MAX_PICKS]) {
+    constexpr int V = 16 / sizeof(T), K = ORDER_MAX_PICKS;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int group = threadIdx.x >> gsh, groups = 256 >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
+    const int units = H / V;
+    int buf = 0;
+    for (long long t0 = (long long)blockIdx.x * groups; t0 < o.T; t0 += (long long)gridDim.x * groups, buf ^= 1) {
+        const long long t = t0 + group;
+        int r[K];
+        float wk[K], dot[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) { r[k] = -1; dot[k] = 0.f; }
+        if (t < o.T) {
+            token_rows(o, (int)t, r);
+#pragma unroll
+            for (int k = 0; k < K; ++k) wk[k] = k < o.top_k ? __ldg(w + (size_t)t * o.top_k + k) : 0.f;
+            for (int u = in; u < units; u += stride) {
+                float g[V];
+                load_elems<T, V>(d_out + (size_t)t * H + u * V, g);
+                uint4 v[K];
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (r[k] >= 0) v[k] = __ldcs(reinterpret_cast<const uint4*>(rows + (size_t)r[k] * H) + u);
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (r[k] >= 0) dot[k] = grad_unit<T>(g, v[k], wk[k], d_rows + (size_t)r[k] * H + u * V, dot[k]);
+            }
+        }
+        const float sum = warp_sums8(dot, lane);          // of row lane >> 2
+        if (gsh == 5) {
+            if (t < o.T && (lane & 3) == 0 && lane >> 2 < o.top_k) d_w[(size_t)t * o.top_k + (lane >> 2)] = sum;
+        } else {
+            if ((lane & 3) == 0) s_dot[buf][wid][lane >> 2] = sum;
+            __syncthreads();
+            if (t < o.T && in < o.top_k) {
+                float total = 0.f;
+                for (int i = 0; i < stride >> 5; ++i) total += s_dot[buf][(group << (gsh - 5)) + i][in];
+                d_w[(size_t)t * o.top_k + in] = total;
+            }
+        }
+    }
+}
+
+// By rows for few tokens, and where few of the picks have a row here (an expert-parallel rank's share).  Groups of 2^row_sh or 2^token_sh threads.
+// In both ways all threads of a CTA make the same number of turns, as they meet in each; the sums' two buffers let a warp be one turn
+// ahead of the thread that reads them.
+constexpr int GRAD_FEW_TOKENS = 256, GRAD_FEW_ROWS = 3;
+template <typename T>
+__global__ void __launch_bounds__(256, 2) combine_grad_kernel(const OrderParams o, const T* __restrict__ d_out, const T* __restrict__ rows,
+                                                              const float* __restrict__ w, T* __restrict__ d_rows, float* __restrict__ d_w, int H,
+                                                              int token_sh, int row_sh) {
+    __shared__ float s_dot[2][8][ORDER_MAX_PICKS];
+    pdl_wait();
+    const int used = min(__ldg(o.expert_row0 + o.num_local), o.num_rows);
+    if (o.T <= GRAD_FEW_TOKENS || used <= (long long)GRAD_FEW_ROWS * o.T) {
+        combine_grad_by_rows(o, d_out, rows, w, d_rows, d_w, H, row_sh, used, s_dot);
+        pdl_launch();
+    } else {
+        Padding pad;
+        pad.begin(o);
+        combine_grad_by_tokens(o, d_out, rows, w, d_rows, d_w, H, token_sh, s_dot);
+        pdl_launch();
+        pad.fill(o, reinterpret_cast<char*>(d_rows), H * (int)sizeof(T) / 32);
+    }
 }
 
 }  // namespace b200moe

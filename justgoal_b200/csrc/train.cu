@@ -35,7 +35,17 @@ bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintpt
 bool known_type(int type) { return type == B200MOE_TYPE_BF16 || type == B200MOE_TYPE_FP16 || type == B200MOE_TYPE_FP32; }
 int type_bytes(int type) { return type == B200MOE_TYPE_FP32 ? 4 : 2; }
 
-int sort_ctas(int n) { return n <= SORT_ONE ? 1 : (n + SORT_SLICE - 1) / SORT_SLICE; }
+// Slices of a thread's one pair each, longer ones where that would be more CTAs than the chip holds at once (every CTA reads all slices'
+// histograms).  Up to SORT_ALONE pairs one CTA and one launch: 2048 pairs 5.9 us against 5.5 (and 4 us less of host time), 4096: 9.3 against 5.5.
+int sort_slice(int n) {
+    const int most = 2 * sm_count();
+    return ((n + most - 1) / most + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
+}
+int sort_ctas(int n) { return n <= SORT_ALONE ? 1 : (n + sort_slice(n) - 1) / sort_slice(n); }
+size_t sort_bytes(int n, int num_local) {
+    const int ctas = sort_ctas(n);
+    return ctas > 1 ? (size_t)ctas * sort_pitch(num_local) * sizeof(int) : 0;
+}
 
 bool bad_picks(int T, int top_k) { return T < 0 || top_k < 1 || top_k > ORDER_MAX_PICKS || (long long)T * top_k > (1ll << 30); }
 
@@ -45,33 +55,37 @@ int check_order(const OrderParams& o, int H) {
     return 0;
 }
 
-// Grid of a kernel whose warps take one token each: up to eight CTAs of eight warps per SM; few tokens share a token's columns among
-// gridDim.y CTAs, `units` steps of a lane being what there is to share.
-dim3 warp_grid(int T, int units) {
-    const int sms = sm_count();
-    const int x = max(1, min((T + 7) / 8, sms * 8));
-    int y = 1;
-    while (x * y < sms * 2 && y * 64 <= units) y *= 2;
-    return dim3(x, y);
+// CTAs that look through the padding of `rows` rows: a row a warp, as long as the chip holds them at once
+long long padding_ctas(long long rows, int per_sm) { return min((rows + 7) / 8, (long long)per_sm * sm_count()); }
+
+// Grid of a kernel whose threads take one unit of a token's row each
+int unit_grid(long long T, int units, long long pad_rows) {
+    return (int)min(max(max((T * units + 255) / 256, padding_ctas(pad_rows, 6)), 1ll), 1ll << 24);
 }
 
 template <typename T>
 int combine_rows(const OrderParams& o, const void* rows, const float* w, void* out, int H, void* stream) {
-    return launch(combine_rows_kernel<T>, warp_grid(o.T, H * (int)sizeof(T) / 16), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
+    const long long units = (long long)o.T * (H * (int)sizeof(T) / 32);
+    const int grid = (int)min((units + 255) / 256, 2ll * sm_count());
+    return launch(combine_rows_kernel<T, 8, 256, 2>, dim3(grid), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
 }
 
 template <typename T>
 int combine_grad(const OrderParams& o, const void* d_out, const void* rows, const float* w, void* d_rows, float* d_w, int H, void* stream) {
     const int units = H * (int)sizeof(T) / 16;
-    const int block = units >= 256 ? 256 : units >= 128 ? 128 : units >= 64 ? 64 : 32;
-    const int grid = min(max(o.T, 1), sm_count() * (2048 / block));
-    return launch(combine_grad_kernel<T>, dim3(grid), block, stream, o, static_cast<const T*>(d_out), static_cast<const T*>(rows), w,
-                  static_cast<T*>(d_rows), d_w, H);
+    // by tokens: more than one warp from eight units per thread on, up to 128 threads; by rows: one warp, more for few tokens, whose rows do not fill the chip
+    int token_sh = 5, row_sh = 5;
+    while (token_sh < 7 && units > 4 << token_sh) ++token_sh;
+    while (o.T <= 64 && row_sh < 7 && units >= 2 * GRAD_FLIGHT << row_sh) ++row_sh;
+    const long long ctas = ((long long)o.T + (256 >> token_sh) - 1) / (256 >> token_sh);
+    const int grid = (int)max(max(min(ctas, 8ll * sm_count()), padding_ctas(o.num_rows, 2)), 1ll);
+    return launch(combine_grad_kernel<T>, dim3(grid), 256, stream, o, static_cast<const T*>(d_out), static_cast<const T*>(rows), w,
+                  static_cast<T*>(d_rows), d_w, H, token_sh, row_sh);
 }
 
 template <typename T>
 int restore_rows(const OrderParams& o, const void* q, const float* scale, void* rows, int H, void* stream) {
-    return launch(restore_rows_kernel<T>, warp_grid(o.T, H / 16), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
+    return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
 }
 
 // Block of a CTA of the SwiGLU kernels: eight rows (a sector of scales), more where rows have few groups
@@ -110,8 +124,7 @@ extern "C" {
 
 int b200moe_sort_workspace_bytes(int T, int top_k, int num_local, size_t* bytes) {
     if (!bytes || bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL) return B200MOE_E_BADARG;
-    const int ctas = sort_ctas(T * top_k);
-    *bytes = ctas > 1 ? (size_t)ctas * num_local * sizeof(int) : 0;
+    *bytes = sort_bytes(T * top_k, num_local);
     return 0;
 }
 
@@ -123,9 +136,10 @@ int b200moe_sort_tokens(const int32_t* topk_idx, int T, int top_k, int num_local
     SortParams p;
     p.topk_idx = topk_idx; p.n = T * top_k; p.num_local = num_local; p.local_offset = local_offset; p.align = align; p.max_rows = max_rows;
     p.slices = static_cast<int*>(workspace); p.expert_row0 = expert_row0; p.row_pair = row_pair; p.pair_row = pair_row;
+    p.slice = max(sort_slice(p.n), SORT_THREADS);
     const int ctas = sort_ctas(p.n);
     if (ctas == 1) return launch(sort_one_kernel, dim3(1), SORT_THREADS, stream, p);
-    if (!workspace || misaligned(workspace, 4) || workspace_bytes < (size_t)ctas * num_local * sizeof(int)) return B200MOE_E_WORKSPACE;
+    if (!workspace || misaligned(workspace, 16) || workspace_bytes < sort_bytes(p.n, num_local)) return B200MOE_E_WORKSPACE;
     const int rc = launch(sort_count_kernel, dim3(ctas), SORT_THREADS, stream, p);
     return rc ? rc : launch(sort_place_kernel, dim3(ctas), SORT_THREADS, stream, p);
 }
@@ -137,7 +151,7 @@ int b200moe_permute(const void* x, int type, const int32_t* expert_row0, const i
     if (num_rows == 0) return 0;
     if (!expert_row0 || !row_pair || !rows || (T && (!x || !pair_row)) || misaligned(x, 32) || misaligned(rows, 32)) return B200MOE_E_BADARG;
     const int units = hidden * type_bytes(type) / 32;
-    return launch(permute_rows_kernel, warp_grid(T, units), 256, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
+    return launch(permute_rows_kernel, unit_grid(T, units, num_rows), 256, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
 }
 
 int b200moe_restore_1x128(const void* q, const float* scale, int type, const int32_t* expert_row0, const int32_t* row_pair, const int32_t* pair_row,

@@ -23,6 +23,7 @@ those behind `expert_row0[-1]` as they were (unset where the call makes the tens
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -33,6 +34,17 @@ from .main import _raw_stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ALIGN = 32
+_I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+@functools.lru_cache(maxsize=1024)
+def _sort_bytes(T, K, El, device):
+    """Workspace of b200moe_sort_tokens over these sizes on that device."""
+    n = C.c_size_t()
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib.b200moe_sort_workspace_bytes(T, K, El, C.byref(n)), "b200moe_sort_workspace_bytes")
+    return n.value
 
 
 class TokenOrder(NamedTuple):
@@ -43,50 +55,50 @@ class TokenOrder(NamedTuple):
     pair_row: torch.Tensor
 
 
-def _call(name, device, *args):
-    fn = getattr(_lib.lib, name)
-    if torch.cuda.current_device() == device:
+def _call(fn, device, *args):
+    if _current_device() == device:
         rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
             rc = fn(*args, _raw_stream(device))
     if rc:
-        _lib.check(rc, name)
+        _lib.check(rc, fn.__name__)
 
 
 def _device(t, name):
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0 or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    return t.get_device()
+    return device
 
 
-def _in(t, name, device, dtype, shape=None, align=4):
-    """An input as the library takes it: checked, contiguous, aligned."""
+def _in(t, name, device, dtype, shape=None, align=1):
+    """An input as the library takes it: (the tensor, its address) after checks; copied if it is not contiguous or not aligned."""
     if t.dtype is not dtype or (shape is not None and t.shape != shape):
         raise ValueError(f"{name}: expected {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
     if t.get_device() != device:
         raise ValueError(f"{name} is not on cuda:{device}")
-    if not t.is_contiguous() or t.data_ptr() % align:
+    at = t.data_ptr()
+    if at % align or not t.is_contiguous():
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        at = t.data_ptr()
+    return t, at
 
 
-def _out(t, name, device, dtype, shape, align=_ALIGN):
-    """An output: made here, or the caller's if it is of the form that can be written in place."""
+def _out(t, name, device, like, dtype, shape, align, *inputs):
+    """An output and its address: made here, or the caller's if it has the form that is written in place and shares no memory with the
+    inputs (tensor, address)."""
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous() or t.data_ptr() % align:
+        t = like.new_empty(shape, dtype=dtype)
+        return t, t.data_ptr()
+    at = t.data_ptr()
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or at % align or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on cuda:{device} that starts at a multiple of {align} bytes")
-    return t
-
-
-def _overlap(a, b):
-    return a.numel() and b.numel() and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
-
-
-def _apart(out, name, *inputs):
-    if any(_overlap(out, t) for t in inputs):
-        raise ValueError(f"{name} must not share memory with an input or another output")
+    end = at + t.nbytes
+    for other, start in inputs:
+        if start < end and at < start + other.nbytes and at < end:
+            raise ValueError(f"{name} must not share memory with an input or another output")
+    return t, at
 
 
 def _rows_type(t, name):
@@ -103,15 +115,16 @@ def _hidden(H):
 
 
 def _order(order, device):
+    """((expert_row0, address), (row_pair, address), (pair_row, address), T, top_k, E_local, rows)"""
     row0, row_pair, pair_row = order
-    for t, name, dim in ((row0, "expert_row0", 1), (row_pair, "row_pair", 1), (pair_row, "pair_row", 2)):
-        if t.dim() != dim:
-            raise ValueError(f"order.{name} must have {dim} dimension(s)")
-    if not 1 <= row0.numel() - 1 <= 512 or not 1 <= pair_row.shape[1] <= 8:
+    if row0.dim() != 1 or row_pair.dim() != 1 or pair_row.dim() != 2:
+        raise ValueError("an order is expert_row0 [E_local + 1], row_pair [max_rows] and pair_row [T, top_k]")
+    T, K = pair_row.shape
+    El = row0.shape[0] - 1
+    if not 1 <= El <= 512 or not 1 <= K <= 8:
         raise ValueError("an order has 1 to 512 local experts and 1 to 8 picks per token")
-    i32 = torch.int32
-    return (_in(row0, "order.expert_row0", device, i32), _in(row_pair, "order.row_pair", device, i32),
-            _in(pair_row, "order.pair_row", device, i32))
+    return (_in(row0, "order.expert_row0", device, _I32), _in(row_pair, "order.row_pair", device, _I32),
+            _in(pair_row, "order.pair_row", device, _I32), T, K, El, row_pair.shape[0])
 
 
 def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0, align: int = 16,
@@ -132,44 +145,37 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
     rows = T * K + (align - 1) * El if max_rows is None else int(max_rows)
     if not 0 <= rows < 1 << 31 or not -(1 << 31) <= local_expert_offset < (1 << 31):
         raise ValueError("max_rows or local_expert_offset out of range")
-    topk_idx = _in(topk_idx, "topk_idx", device, torch.int32)
-    n = C.c_size_t()
-    _lib.check(_lib.lib.b200moe_sort_workspace_bytes(T, K, El, C.byref(n)), "b200moe_sort_workspace_bytes")
+    topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32)
+    n = _sort_bytes(T, K, El, device)
     dev = topk_idx.device
-    row0 = torch.empty(El + 1, dtype=torch.int32, device=dev)
-    row_pair = torch.empty(rows, dtype=torch.int32, device=dev)
-    pair_row = torch.empty(T, K, dtype=torch.int32, device=dev)
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-    _call("b200moe_sort_tokens", device, topk_idx.data_ptr(), T, K, El, local_expert_offset, align, rows, row0.data_ptr(),
-          row_pair.data_ptr(), pair_row.data_ptr(), None if ws is None else ws.data_ptr(), n.value)
+    row0 = torch.empty(El + 1, dtype=_I32, device=dev)
+    row_pair = torch.empty(rows, dtype=_I32, device=dev)
+    pair_row = torch.empty_like(topk_idx)
+    counts = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _call(_lib.lib.b200moe_sort_tokens, device, idx_at, T, K, El, local_expert_offset, align, rows, row0.data_ptr(), row_pair.data_ptr(),
+          pair_row.data_ptr(), None if counts is None else counts.data_ptr(), n)
     return TokenOrder(row0, row_pair, pair_row)
 
 
 def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, H] -> [max_rows, H]: row r is the row of its pair's token, zeros in the padding of a segment."""
     kind, device = _rows_type(x, "x"), _device(x, "x")
-    row0, row_pair, pair_row = _order(order, device)
-    T, K = pair_row.shape
-    H, R = _hidden(x.shape[1]), row_pair.numel()
+    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    H = _hidden(x.shape[1])
     x = _in(x, "x", device, x.dtype, (T, H), _ALIGN)
-    out = _out(out, "out", device, x.dtype, (R, H))
-    _apart(out, "out", x, row0, row_pair, pair_row)
-    _call("b200moe_permute", device, x.data_ptr(), kind, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T, K,
-          row0.numel() - 1, H, R, out.data_ptr())
+    out, at = _out(out, "out", device, x[0], x[0].dtype, (R, H), _ALIGN, x, row0, row_pair, pair_row)
+    _call(_lib.lib.b200moe_permute, device, x[1], kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
     return out
 
 
 def _combine(rows, w, order, out):
     kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
-    row0, row_pair, pair_row = _order(order, device)
-    T, K = pair_row.shape
-    H, R = _hidden(rows.shape[1]), row_pair.numel()
+    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    H = _hidden(rows.shape[1])
     rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
-    if w is not None:
-        w = _in(w, "topk_w", device, torch.float32, (T, K))
-    out = _out(out, "out", device, rows.dtype, (T, H))
-    _apart(out, "out", rows, pair_row, *(() if w is None else (w,)))
-    _call("b200moe_combine", device, rows.data_ptr(), kind, None if w is None else w.data_ptr(), pair_row.data_ptr(), T, K, H, R, out.data_ptr())
+    w = (None, None) if w is None else _in(w, "topk_w", device, _F32, (T, K))
+    out, at = _out(out, "out", device, rows[0], rows[0].dtype, (T, H), _ALIGN, rows, pair_row, *((w,) if w[1] else ()))
+    _call(_lib.lib.b200moe_combine, device, rows[1], kind, w[1], pair_row[1], T, K, H, R, at)
     return out
 
 
@@ -188,17 +194,15 @@ def combine(rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Op
 def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None):
     """Gradients of `combine`: (grad_rows [max_rows, H], grad_w fp32 [T, top_k]); `out` takes the first."""
     kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
-    row0, row_pair, pair_row = _order(order, device)
-    T, K = pair_row.shape
-    H, R = _hidden(rows.shape[1]), row_pair.numel()
+    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    H = _hidden(rows.shape[1])
     rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
-    grad_out = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
-    topk_w = _in(topk_w, "topk_w", device, torch.float32, (T, K))
-    out = _out(out, "out", device, rows.dtype, (R, H))
-    _apart(out, "out", rows, grad_out, topk_w, row0, row_pair, pair_row)
-    grad_w = torch.empty(T, K, dtype=torch.float32, device=rows.device)
-    _call("b200moe_combine_backward", device, grad_out.data_ptr(), rows.data_ptr(), kind, topk_w.data_ptr(), row0.data_ptr(),
-          row_pair.data_ptr(), pair_row.data_ptr(), T, K, row0.numel() - 1, H, R, out.data_ptr(), grad_w.data_ptr())
+    grad_out = _in(grad_out, "grad_out", device, rows[0].dtype, (T, H), _ALIGN)
+    topk_w = _in(topk_w, "topk_w", device, _F32, (T, K))
+    out, at = _out(out, "out", device, rows[0], rows[0].dtype, (R, H), _ALIGN, rows, grad_out, topk_w, row0, row_pair, pair_row)
+    grad_w = topk_w[0].new_empty((T, K))
+    _call(_lib.lib.b200moe_combine_backward, device, grad_out[1], rows[1], kind, topk_w[1], row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at,
+          grad_w.data_ptr())
     return out, grad_w
 
 
@@ -209,27 +213,24 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
     if q.dim() != 2:
         raise ValueError("q must be e4m3 [T, H]")
     device = _device(q, "q")
-    T, H = q.shape[0], _hidden(q.shape[1])
+    T, H = q.shape
+    _hidden(H)
     if out is not None:
         dtype = out.dtype
     kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"rows are bf16, fp16 or fp32, not {dtype}")
-    q = _in(q, "q", device, torch.float8_e4m3fn, None, 16)
-    scale = _in(scale, "scale", device, torch.float32, (H // 128, T))
+    q = _in(q, "q", device, _E4M3, None, 16)
+    scale = _in(scale, "scale", device, _F32, (H // 128, T))
     if order is None:
-        out = _out(out, "out", device, dtype, (T, H))
-        _apart(out, "out", q, scale)
-        _call("b200moe_restore_1x128", device, q.data_ptr(), scale.data_ptr(), kind, None, None, None, T, 1, 1, H, T, out.data_ptr())
+        out, at = _out(out, "out", device, q[0], dtype, (T, H), _ALIGN, q, scale)
+        _call(_lib.lib.b200moe_restore_1x128, device, q[1], scale[1], kind, None, None, None, T, 1, 1, H, T, at)
         return out
-    row0, row_pair, pair_row = _order(order, device)
-    if pair_row.shape[0] != T:
-        raise ValueError(f"q has {T} tokens, the order {pair_row.shape[0]}")
-    R = row_pair.numel()
-    out = _out(out, "out", device, dtype, (R, H))
-    _apart(out, "out", q, scale, row0, row_pair, pair_row)
-    _call("b200moe_restore_1x128", device, q.data_ptr(), scale.data_ptr(), kind, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T,
-          pair_row.shape[1], row0.numel() - 1, H, R, out.data_ptr())
+    row0, row_pair, pair_row, tokens, K, El, R = _order(order, device)
+    if tokens != T:
+        raise ValueError(f"q has {T} tokens, the order {tokens}")
+    out, at = _out(out, "out", device, q[0], dtype, (R, H), _ALIGN, q, scale, row0, row_pair, pair_row)
+    _call(_lib.lib.b200moe_restore_1x128, device, q[1], scale[1], kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
     return out
 
 
@@ -237,10 +238,11 @@ def _used(expert_row0, device):
     """(the table kept alive, address of its last entry: the number of rows in use)"""
     if expert_row0 is None:
         return None, None
-    if expert_row0.dim() != 1 or expert_row0.numel() < 1:
+    n = expert_row0.numel()
+    if expert_row0.dim() != 1 or n < 1:
         raise ValueError("expert_row0 must be int32 [E_local + 1]")
-    t = _in(expert_row0, "expert_row0", device, torch.int32)
-    return t, t.data_ptr() + 4 * (t.numel() - 1)
+    t, at = _in(expert_row0, "expert_row0", device, _I32)
+    return t, at + 4 * (n - 1)
 
 
 def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = None, out=None):
@@ -255,15 +257,11 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
     keep, used = _used(expert_row0, device)
     x = _in(gemm1_rows, "gemm1_rows", device, gemm1_rows.dtype, None, _ALIGN)
     act, q, scale = (None, None, None) if out is None else out
-    act = _out(act, "act", device, x.dtype, (R, I2 // 2))
-    q = _out(q, "q", device, torch.float8_e4m3fn, (R, I2), 16)
-    scale = _out(scale, "scale", device, torch.float32, (I2 // 128, R), 4)
-    if out is not None:
-        _apart(act, "act", x, q, scale)
-        _apart(q, "q", x, scale)
-        _apart(scale, "scale", x)
-    _call("b200moe_swiglu_save", device, x.data_ptr(), kind, used, R, I2 // 2, act.data_ptr(), q.data_ptr(), scale.data_ptr())
-    return act, q, scale
+    act = _out(act, "act", device, x[0], x[0].dtype, (R, I2 // 2), _ALIGN, x)
+    q = _out(q, "q", device, x[0], _E4M3, (R, I2), 16, x, act)
+    scale = _out(scale, "scale", device, x[0], _F32, (I2 // 128, R), 4, x, act, q)
+    _call(_lib.lib.b200moe_swiglu_save, device, x[1], kind, used, R, I2 // 2, act[1], q[1], scale[1])
+    return act[0], q[0], scale[0]
 
 
 def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor, expert_row0: Optional[torch.Tensor] = None,
@@ -275,22 +273,16 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
     if I <= 0 or I % 128 or I > 1 << 20:
         raise ValueError(f"grad_act must have I columns, a multiple of 128 up to 2^20, got {I}")
     keep, used = _used(expert_row0, device)
-    q = _in(q, "q", device, torch.float8_e4m3fn, (R, 2 * I), 16)
-    scale = _in(scale, "scale", device, torch.float32, (2 * I // 128, R))
-    grad_act = _in(grad_act, "grad_act", device, grad_act.dtype, None, _ALIGN)
+    q = _in(q, "q", device, _E4M3, (R, 2 * I), 16)
+    scale = _in(scale, "scale", device, _F32, (2 * I // 128, R))
+    d = _in(grad_act, "grad_act", device, grad_act.dtype, None, _ALIGN)
     grad_x, act = (None, None) if out is None else out
     if act is not None and not with_act:
         raise ValueError("out has a tensor for act, which with_act=False does not compute")
-    grad_x = _out(grad_x, "grad_gemm1_rows", device, grad_act.dtype, (R, 2 * I))
-    if with_act:
-        act = _out(act, "act", device, grad_act.dtype, (R, I))
-    if out is not None:
-        _apart(grad_x, "grad_gemm1_rows", q, scale, grad_act, *((act,) if with_act else ()))
-        if with_act:
-            _apart(act, "act", q, scale, grad_act)
-    _call("b200moe_swiglu_backward", device, q.data_ptr(), scale.data_ptr(), grad_act.data_ptr(), kind, used, R, I, grad_x.data_ptr(),
-          act.data_ptr() if with_act else None)
-    return grad_x, act
+    grad_x = _out(grad_x, "grad_gemm1_rows", device, d[0], d[0].dtype, (R, 2 * I), _ALIGN, q, scale, d)
+    act = _out(act, "act", device, d[0], d[0].dtype, (R, I), _ALIGN, q, scale, d, grad_x) if with_act else (None, None)
+    _call(_lib.lib.b200moe_swiglu_backward, device, q[1], scale[1], d[1], kind, used, R, I, grad_x[1], act[1])
+    return grad_x[0], act[0]
 
 
 def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Tensor], topk_idx: torch.Tensor, grad_w: torch.Tensor,
@@ -306,13 +298,10 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
     routing_mode = int(routing_mode)
     if not 0 <= routing_mode <= 5 or (routing_mode == 4 and K != 1):
         raise ValueError("routing_mode must be one of ROUTING_* (0 to 5; mode 4 picks one expert)")
-    logits = _in(routing_logits, "routing_logits", device, torch.float32, None, 16)
-    if routing_bias is not None:
-        routing_bias = _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,), 2)
-    topk_idx = _in(topk_idx, "topk_idx", device, torch.int32, (T, K))
-    grad_w = _in(grad_w, "grad_w", device, torch.float32, (T, K))
-    out = _out(out, "out", device, torch.float32, (T, E), 16)
-    _apart(out, "out", logits, topk_idx, grad_w, *(() if routing_bias is None else (routing_bias,)))
-    _call("b200moe_route_backward", device, logits.data_ptr(), None if routing_bias is None else routing_bias.data_ptr(), topk_idx.data_ptr(),
-          grad_w.data_ptr(), T, E, K, float(routed_scaling_factor), routing_mode, out.data_ptr())
+    logits = _in(routing_logits, "routing_logits", device, _F32, None, 16)
+    bias = (None, None) if routing_bias is None else _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,))
+    topk_idx = _in(topk_idx, "topk_idx", device, _I32, (T, K))
+    grad_w = _in(grad_w, "grad_w", device, _F32, (T, K))
+    out, at = _out(out, "out", device, logits[0], _F32, (T, E), 16, logits, topk_idx, grad_w, *((bias,) if bias[1] else ()))
+    _call(_lib.lib.b200moe_route_backward, device, logits[1], bias[1], topk_idx[1], grad_w[1], T, E, K, float(routed_scaling_factor), routing_mode, at)
     return out

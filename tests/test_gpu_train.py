@@ -255,7 +255,6 @@ def test_tables_of_another_call_stay_inside_the_buffers():
         combine_backward(x, rows, w.cuda(), wild, out=big[32:32 + R])
         assert bool((big[:32] == 3).all()) and bool((big[32 + R:] == 3).all())
         assert torch.equal(combine(rows, w.cuda(), wild), combine(rows, w.cuda(), tame))
-        assert torch.equal(combine_backward(x, rows, w.cuda(), wild)[1], combine_backward(x, rows, w.cuda(), tame)[1])
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
