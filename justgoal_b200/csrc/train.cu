@@ -88,12 +88,19 @@ int restore_rows(const OrderParams& o, const void* q, const float* scale, void* 
     return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
 }
 
-// Block of a CTA of the SwiGLU kernels: eight rows (a sector of scales), more where rows have few groups
+// Block of a CTA of the SwiGLU kernels: the fewest rows, four or eight at least, that keep the CTA's threads busy in nearly all of its turns (40000 x
+// 640, five groups: eight rows 44.3 us, 16: 39.4), fewer where that leaves less than two CTAs per SM.  Eight / four rows where both do
+// (2048 columns; save, backward): 2000 rows 9.7 / 7.4 us, 10.7 / 10.0, 8000: 25.1 / 24.3, 30.0 / 28.4, 34645: 90.9 / 90.7, 109.7 / 111.6;
+// so eight from 16 CTAs per SM on.
 void swiglu_block(int rows, int I, int& rsh, int& gpc, dim3& grid) {
     const int groups = I >> 7, parts = (groups + 63) / 64;
     gpc = (groups + parts - 1) / parts;
-    rsh = 3;
-    while ((gpc << rsh) < SWIGLU_TURN) ++rsh;
+    rsh = ((long long)rows >> 3) * parts >= 16ll * sm_count() ? 3 : 2;
+    while (rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES) {
+        const int items = gpc << rsh, turns = (items + SWIGLU_TURN - 1) / SWIGLU_TURN;
+        if (items * 10 >= turns * SWIGLU_TURN * 9) break;
+        ++rsh;
+    }
     while (rsh > 0 && (long long)((rows + (1 << rsh) - 1) >> rsh) * parts < 2ll * sm_count()) --rsh;
     grid = dim3((rows + (1 << rsh) - 1) >> rsh, (groups + gpc - 1) / gpc);
 }
@@ -209,18 +216,21 @@ int b200moe_swiglu_backward(const void* q, const float* scale, const void* grad_
 
 int b200moe_route_backward(const float* routing_logits, const void* routing_bias, const int32_t* topk_idx, const float* grad_w, int T, int num_experts,
                            int top_k, float routed_scaling_factor, int routing_mode, float* grad_logits, void* stream) {
-    if (bad_picks(T, top_k) || num_experts < 32 || num_experts > 128 * ROUTE_GRAD_COLS || num_experts % 32 || top_k > num_experts) return B200MOE_E_BADARG;
+    if (bad_picks(T, top_k) || num_experts < 32 || num_experts > ROUTE_GRAD_MAX || num_experts % 32 || top_k > num_experts) return B200MOE_E_BADARG;
     if (routing_mode < 0 || routing_mode >= RG_COUNT || (routing_mode == RG_LLAMA4 && top_k != 1)) return B200MOE_E_BADARG;
     if (T == 0) return 0;
     if (!routing_logits || !topk_idx || !grad_w || !grad_logits || misaligned(routing_logits, 16) || misaligned(grad_logits, 16)) return B200MOE_E_BADARG;
     const RouteGradParams p = {routing_logits, static_cast<const __nv_bfloat16*>(routing_bias), topk_idx, grad_w, grad_logits, T, num_experts, top_k,
                                routed_scaling_factor};
-    auto* kern = routing_mode == RG_DEEPSEEK  ? route_grad_kernel<RG_DEEPSEEK>
-                 : routing_mode == RG_DEFAULT ? route_grad_kernel<RG_DEFAULT>
-                 : routing_mode == RG_LLAMA4  ? route_grad_kernel<RG_LLAMA4>
-                 : routing_mode == RG_TOPK    ? route_grad_kernel<RG_TOPK>
-                                              : route_grad_kernel<RG_RENORMALIZE>;
-    return launch(kern, dim3((T + 7) / 8), 256, stream, p);
+    if (routing_mode == RG_DEFAULT) {
+        auto* kern = num_experts <= 128 ? route_grad_softmax_kernel<1> : num_experts <= 256 ? route_grad_softmax_kernel<2> : route_grad_softmax_kernel<4>;
+        return launch(kern, dim3((T + 7) / 8), 256, stream, p);
+    }
+    auto* kern = routing_mode == RG_DEEPSEEK ? route_grad_kernel<RG_DEEPSEEK>
+                 : routing_mode == RG_LLAMA4 ? route_grad_kernel<RG_LLAMA4>
+                 : routing_mode == RG_TOPK   ? route_grad_kernel<RG_TOPK>
+                                             : route_grad_kernel<RG_RENORMALIZE>;
+    return launch(kern, dim3((T + 31) / 32), 256, stream, p);
 }
 
 }  // extern "C"
