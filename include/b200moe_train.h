@@ -7,7 +7,7 @@
  * the caller passes to both.  Return values as in b200moe.h.
  *
  * T tokens with top_k picks each (top_k <= 8, T * top_k <= 2^30); pair i = t * top_k + k; num_local experts (<= 512); hidden and
- * intermediate are multiples of 128.  All data pointers are device pointers; inputs are not modified, outputs overlap neither inputs
+ * intermediate are multiples of 128 up to 2^20, row tensors have up to 2^30 rows.  All data pointers are device pointers; inputs are not modified, outputs overlap neither inputs
  * nor each other.  Row tensors have one of the three types below and start at a multiple of 32 bytes, e4m3 tensors at 16.  Sums
  * are fp32 in a fixed order with one rounding: results are the same from run to run.
  * (No counterpart in the reference, which has no backward pass.)

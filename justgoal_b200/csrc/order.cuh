@@ -276,13 +276,22 @@ __device__ __forceinline__ Unit unit_of(unsigned long long g, unsigned units) {
     return {(int)t, (int)(g - (unsigned long long)t * units)};
 }
 
-// Rows of token t, -1 where a pick has none
+// Rows of token t, -1 where a pick has none.  (Four picks per load where the table allows it.)
 __device__ __forceinline__ void token_rows(const OrderParams& o, int t, int* r) {
+    const int32_t* src = o.pair_row + (size_t)t * o.top_k;
+    if (o.top_k % 4 == 0 && (reinterpret_cast<uintptr_t>(o.pair_row) & 15) == 0) {
 #pragma unroll
-    for (int k = 0; k < ORDER_MAX_PICKS; ++k) {
-        r[k] = k < o.top_k ? __ldg(o.pair_row + (size_t)t * o.top_k + k) : -1;
-        if (r[k] >= o.num_rows) r[k] = -1;
+        for (int k = 0; k < ORDER_MAX_PICKS; k += 4) {
+            const int4 q = k < o.top_k ? __ldg(reinterpret_cast<const int4*>(src + k)) : make_int4(-1, -1, -1, -1);
+            r[k] = q.x; r[k + 1] = q.y; r[k + 2] = q.z; r[k + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < ORDER_MAX_PICKS; ++k) r[k] = k < o.top_k ? __ldg(src + k) : -1;
     }
+#pragma unroll
+    for (int k = 0; k < ORDER_MAX_PICKS; ++k)
+        if (r[k] >= o.num_rows) r[k] = -1;
 }
 
 // Zeros into the padding rows of the segments.  Every warp owns a block of up to 32 consecutive rows (several where there are more rows than
@@ -376,10 +385,10 @@ __global__ void __launch_bounds__(256) restore_rows_kernel(const OrderParams o, 
 
 // ---------------------------------------------------------------- rows back to their tokens
 // out[t] = sum_k w[t, k] rows[r(t, k)], w null: ones.  A thread takes 32-byte units, one after the other: while the rows of one are on their
-// way it looks up the rows of the next, so that the chain of dependent loads is paid once.  FLIGHT rows' loads are in flight together.
-template <typename T, int FLIGHT, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
-                                                                     T* __restrict__ out, int H) {
+// way it looks up the rows of the next, so that the chain of dependent loads is paid once; up to eight rows' loads are in flight.
+template <typename T>
+__global__ void __launch_bounds__(256, 2) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
+                                                              T* __restrict__ out, int H) {
     constexpr int V = 32 / sizeof(T), K = ORDER_MAX_PICKS;
     pdl_wait();
     const int units = H / V;
@@ -393,36 +402,32 @@ __global__ void __launch_bounds__(THREADS, CTAS) combine_rows_kernel(const Order
             const unsigned long long next = g + step;
             Unit at2 = {0, 0};
             int r2[K];
-            float acc[V];
+            uint32_t v[K][8];
+            float wk[K], acc[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
 #pragma unroll
-            for (int k0 = 0; k0 < K; k0 += FLIGHT) {
-                uint32_t v[FLIGHT][8];
-                float wk[FLIGHT];
-#pragma unroll
-                for (int k = 0; k < FLIGHT; ++k)
-                    if (r[k0 + k] >= 0) {
-                        ld_global_v8(rows + (size_t)r[k0 + k] * H + at.unit * V, v[k]);
-                        wk[k] = w ? __ldg(w + (size_t)at.token * o.top_k + k0 + k) : 1.f;
-                    }
-                if (k0 + FLIGHT == K && next < total) {
-                    at2 = unit_of(next, units);
-                    token_rows(o, at2.token, r2);
+            for (int k = 0; k < K; ++k)
+                if (r[k] >= 0) {
+                    ld_global_v8(rows + (size_t)r[k] * H + at.unit * V, v[k]);
+                    wk[k] = w ? __ldg(w + (size_t)at.token * o.top_k + k) : 1.f;
                 }
-#pragma unroll
-                for (int k = 0; k < FLIGHT; ++k)
-                    if (r[k0 + k] >= 0)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if constexpr (sizeof(T) == 4) {
-                                acc[i] = fmaf(wk[k], __uint_as_float(v[k][i]), acc[i]);
-                            } else {
-                                const float2 f = Elem<T>::unpack(v[k][i]);
-                                acc[2 * i] = fmaf(wk[k], f.x, acc[2 * i]); acc[2 * i + 1] = fmaf(wk[k], f.y, acc[2 * i + 1]);
-                            }
-                        }
+            if (next < total) {
+                at2 = unit_of(next, units);
+                token_rows(o, at2.token, r2);
             }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (r[k] >= 0)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (sizeof(T) == 4) {
+                            acc[i] = fmaf(wk[k], __uint_as_float(v[k][i]), acc[i]);
+                        } else {
+                            const float2 f = Elem<T>::unpack(v[k][i]);
+                            acc[2 * i] = fmaf(wk[k], f.x, acc[2 * i]); acc[2 * i + 1] = fmaf(wk[k], f.y, acc[2 * i + 1]);
+                        }
+                    }
             store_elems<T, V>(out + g * V, acc);
             if (next >= total) break;
             g = next; at = at2;
@@ -499,13 +504,14 @@ __device__ __forceinline__ void combine_grad_by_rows(const OrderParams& o, const
         if (r < 0 || r >= o.num_rows) d_w[i] = 0.f;
     }
     int buf = 0;
-    for (long long r0 = (long long)blockIdx.x * groups; r0 < used; r0 += (long long)gridDim.x * groups, buf ^= 1) {
+    const long long step = (long long)gridDim.x * groups, r_first = (long long)blockIdx.x * groups + (threadIdx.x >> gsh);
+    int next = r_first < used ? __ldg(o.row_pair + r_first) : -1;          // the next row's pair, looked up one turn ahead
+    for (long long r0 = (long long)blockIdx.x * groups; r0 < used; r0 += step, buf ^= 1) {
         const long long r = r0 + (threadIdx.x >> gsh);
-        int pair = -1;
+        const int pair = next < pairs ? next : -1;
+        next = r + step < used ? __ldg(o.row_pair + r + step) : -1;
         float dot = 0.f;
         if (r < used) {
-            pair = __ldg(o.row_pair + r);
-            if (pair >= pairs) pair = -1;
             T* dst = d_rows + (size_t)r * H;
             if (pair < 0) {
                 for (int u = in; u < units / 2; u += stride) st_global_v8(reinterpret_cast<char*>(dst) + (size_t)u * 32, 0, 0, 0, 0, 0, 0, 0, 0);

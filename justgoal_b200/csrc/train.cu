@@ -47,11 +47,15 @@ size_t sort_bytes(int n, int num_local) {
     return ctas > 1 ? (size_t)ctas * sort_pitch(num_local) * sizeof(int) : 0;
 }
 
+constexpr int MAX_COLUMNS = 1 << 20, MAX_ROWS = 1 << 30;      // (index arithmetic stays in range; far above what a GPU's memory holds)
+
 bool bad_picks(int T, int top_k) { return T < 0 || top_k < 1 || top_k > ORDER_MAX_PICKS || (long long)T * top_k > (1ll << 30); }
 
 // The sizes and tables that the row kernels share
 int check_order(const OrderParams& o, int H) {
-    if (bad_picks(o.T, o.top_k) || o.num_local < 1 || o.num_local > ORDER_MAX_LOCAL || o.num_rows < 0 || H <= 0 || H % 128) return B200MOE_E_BADARG;
+    if (bad_picks(o.T, o.top_k) || o.num_local < 1 || o.num_local > ORDER_MAX_LOCAL || o.num_rows < 0 || o.num_rows > MAX_ROWS || H <= 0 ||
+        H % 128 || H > MAX_COLUMNS)
+        return B200MOE_E_BADARG;
     return 0;
 }
 
@@ -67,7 +71,7 @@ template <typename T>
 int combine_rows(const OrderParams& o, const void* rows, const float* w, void* out, int H, void* stream) {
     const long long units = (long long)o.T * (H * (int)sizeof(T) / 32);
     const int grid = (int)min((units + 255) / 256, 2ll * sm_count());
-    return launch(combine_rows_kernel<T, 8, 256, 2>, dim3(grid), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
+    return launch(combine_rows_kernel<T>, dim3(grid), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
 }
 
 template <typename T>
@@ -137,7 +141,8 @@ int b200moe_sort_workspace_bytes(int T, int top_k, int num_local, size_t* bytes)
 
 int b200moe_sort_tokens(const int32_t* topk_idx, int T, int top_k, int num_local, int local_offset, int align, int max_rows,
                         int32_t* expert_row0, int32_t* row_pair, int32_t* pair_row, void* workspace, size_t workspace_bytes, void* stream) {
-    if (bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL || align < 1 || align > 128 || (align & (align - 1)) || max_rows < 0)
+    if (bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL || align < 1 || align > 128 || (align & (align - 1)) || max_rows < 0 ||
+        max_rows > MAX_ROWS)
         return B200MOE_E_BADARG;
     if (!expert_row0 || (max_rows && !row_pair) || (T && (!topk_idx || !pair_row))) return B200MOE_E_BADARG;
     SortParams p;
@@ -170,7 +175,7 @@ int b200moe_restore_1x128(const void* q, const float* scale, int type, const int
         if (num_rows == 0) return 0;
         if (!expert_row0 || !row_pair || !rows || (T && (!q || !scale || !pair_row))) return B200MOE_E_BADARG;
     } else {
-        if (T < 0 || hidden <= 0 || hidden % 128) return B200MOE_E_BADARG;
+        if (T < 0 || T > MAX_ROWS || hidden <= 0 || hidden % 128 || hidden > MAX_COLUMNS) return B200MOE_E_BADARG;
         if (T == 0) return 0;
         if (!q || !scale || !rows) return B200MOE_E_BADARG;
     }
@@ -199,7 +204,8 @@ int b200moe_combine_backward(const void* grad_out, const void* rows, int type, c
 
 int b200moe_swiglu_save(const void* gemm1_rows, int type, const int32_t* used_rows, int num_rows, int intermediate, void* act, void* q, float* scale,
                         void* stream) {
-    if (!known_type(type) || num_rows < 0 || intermediate <= 0 || intermediate % 128 || intermediate > (1 << 20)) return B200MOE_E_BADARG;
+    if (!known_type(type) || num_rows < 0 || num_rows > MAX_ROWS || intermediate <= 0 || intermediate % 128 || intermediate > MAX_COLUMNS)
+        return B200MOE_E_BADARG;
     if (num_rows == 0) return 0;
     if (!gemm1_rows || !act || !q || !scale || misaligned(gemm1_rows, 32) || misaligned(act, 32) || misaligned(q, 16)) return B200MOE_E_BADARG;
     return BY_TYPE(swiglu_save)(gemm1_rows, used_rows, num_rows, intermediate, act, q, scale, stream);
@@ -207,7 +213,8 @@ int b200moe_swiglu_save(const void* gemm1_rows, int type, const int32_t* used_ro
 
 int b200moe_swiglu_backward(const void* q, const float* scale, const void* grad_act, int type, const int32_t* used_rows, int num_rows, int intermediate,
                             void* grad_gemm1_rows, void* act, void* stream) {
-    if (!known_type(type) || num_rows < 0 || intermediate <= 0 || intermediate % 128 || intermediate > (1 << 20)) return B200MOE_E_BADARG;
+    if (!known_type(type) || num_rows < 0 || num_rows > MAX_ROWS || intermediate <= 0 || intermediate % 128 || intermediate > MAX_COLUMNS)
+        return B200MOE_E_BADARG;
     if (num_rows == 0) return 0;
     if (!q || !scale || !grad_act || !grad_gemm1_rows) return B200MOE_E_BADARG;
     if (misaligned(q, 16) || misaligned(grad_act, 32) || misaligned(grad_gemm1_rows, 32) || misaligned(act, 32)) return B200MOE_E_BADARG;

@@ -143,7 +143,7 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
     if align not in (1, 2, 4, 8, 16, 32, 64, 128):
         raise ValueError("align must be a power of two up to 128")
     rows = T * K + (align - 1) * El if max_rows is None else int(max_rows)
-    if not 0 <= rows < 1 << 31 or not -(1 << 31) <= local_expert_offset < (1 << 31):
+    if not 0 <= rows <= 1 << 30 or not -(1 << 31) <= local_expert_offset < (1 << 31):
         raise ValueError("max_rows or local_expert_offset out of range")
     topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32)
     n = _sort_bytes(T, K, El, device)

@@ -51,6 +51,7 @@ def _row_calls(type=0, T=4, K=8, El=32, H=128, R=100, x=P, row0=P, row_pair=P, p
 
 
 @pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(T=-1), dict(K=0), dict(K=9), dict(H=0), dict(H=100), dict(H=-128), dict(R=-1),
+                                 dict(H=(1 << 20) + 128), dict(R=(1 << 30) + 1),
                                  dict(T=1 << 28), dict(pair_row=None), dict(rows=None), dict(rows=ODD)])
 def test_row_operators_refuse(bad):
     assert _row_calls(**bad) == [-1] * 4
@@ -89,7 +90,7 @@ def test_swiglu_refuses():
         a = {**good, **kw}
         return lib.b200moe_swiglu_backward(a["q"], a["scale"], a["x"], a["type"], a["used"], a["R"], a["I"], a["gx"] if "gx" in kw else P, a["act"], None)
 
-    for bad in (dict(type=3), dict(R=-1), dict(I=0), dict(I=100), dict(I=(1 << 20) + 128), dict(x=None), dict(x=ODD), dict(q=None), dict(q=ODD),
+    for bad in (dict(type=3), dict(R=-1), dict(R=(1 << 30) + 1), dict(I=0), dict(I=100), dict(I=(1 << 20) + 128), dict(x=None), dict(x=ODD), dict(q=None), dict(q=ODD),
                 dict(scale=None), dict(act=ODD)):
         assert save(**bad) == -1 and grad(**bad) == -1, bad
     assert save(act=None) == -1 and grad(gx=None) == -1 and grad(gx=ODD) == -1
