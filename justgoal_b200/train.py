@@ -67,15 +67,19 @@ def _call(fn, device, *args):
 
 def _device(t, name):
     device = t.get_device()
-    if device < 0 or not t.is_cuda:
+    if device < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
     return device
 
 
-def _in(t, name, device, dtype, shape=None, align=1):
-    """An input as the library takes it: (the tensor, its address) after checks; copied if it is not contiguous or not aligned."""
-    if t.dtype is not dtype or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name}: expected {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
+def _shape(t, name, shape, dtype):
+    raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _in(t, name, device, dtype, shape, align=1):
+    """An input of a known form: (the tensor, its address); copied if it is not contiguous or not aligned."""
+    if t.dtype is not dtype or t.shape != shape:
+        _shape(t, name, shape, dtype)
     if t.get_device() != device:
         raise ValueError(f"{name} is not on cuda:{device}")
     at = t.data_ptr()
@@ -83,6 +87,22 @@ def _in(t, name, device, dtype, shape=None, align=1):
         t = t.clone(memory_format=torch.contiguous_format)
         at = t.data_ptr()
     return t, at
+
+
+def _rows(t, name, columns=128):
+    """A row tensor that tells the call's type, device and sizes: (the tensor, its address, type, device, rows, columns)."""
+    kind = _TYPES.get(t.dtype)
+    if kind is None or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
+    device = _device(t, name)
+    n, H = t.shape
+    if H <= 0 or H % columns or H > columns << 13:
+        raise ValueError(f"{name}: columns must be a multiple of {columns} up to {columns << 13}, got {H}")
+    at = t.data_ptr()
+    if at % _ALIGN or not t.is_contiguous():
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = t.data_ptr()
+    return t, at, kind, device, n, H
 
 
 def _out(t, name, device, like, dtype, shape, align, *inputs):
@@ -101,30 +121,19 @@ def _out(t, name, device, like, dtype, shape, align, *inputs):
     return t, at
 
 
-def _rows_type(t, name):
-    kind = _TYPES.get(t.dtype)
-    if kind is None or t.dim() != 2:
-        raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
-    return kind
-
-
-def _hidden(H):
-    if H <= 0 or H % 128:
-        raise ValueError(f"columns must be a multiple of 128, got {H}")
-    return H
-
-
 def _order(order, device):
-    """((expert_row0, address), (row_pair, address), (pair_row, address), T, top_k, E_local, rows)"""
+    """An order's ((expert_row0, address), (row_pair, address), (pair_row, address), T, top_k, E_local, rows)."""
     row0, row_pair, pair_row = order
-    if row0.dim() != 1 or row_pair.dim() != 1 or pair_row.dim() != 2:
-        raise ValueError("an order is expert_row0 [E_local + 1], row_pair [max_rows] and pair_row [T, top_k]")
+    if not (row0.dtype is _I32 and row_pair.dtype is _I32 and pair_row.dtype is _I32 and row0.dim() == 1 and row_pair.dim() == 1
+            and pair_row.dim() == 2 and row0.get_device() == device and row_pair.get_device() == device and pair_row.get_device() == device):
+        raise ValueError(f"an order is int32 expert_row0 [E_local + 1], row_pair [max_rows] and pair_row [T, top_k] on cuda:{device}")
+    if not (row0.is_contiguous() and row_pair.is_contiguous() and pair_row.is_contiguous()):
+        row0, row_pair, pair_row = row0.contiguous(), row_pair.contiguous(), pair_row.contiguous()
     T, K = pair_row.shape
-    El = row0.shape[0] - 1
-    if not 1 <= El <= 512 or not 1 <= K <= 8:
+    El = row0.numel() - 1
+    if not (1 <= El <= 512 and 1 <= K <= 8):
         raise ValueError("an order has 1 to 512 local experts and 1 to 8 picks per token")
-    return (_in(row0, "order.expert_row0", device, _I32), _in(row_pair, "order.row_pair", device, _I32),
-            _in(pair_row, "order.pair_row", device, _I32), T, K, El, row_pair.shape[0])
+    return (row0, row0.data_ptr()), (row_pair, row_pair.data_ptr()), (pair_row, pair_row.data_ptr()), T, K, El, row_pair.numel()
 
 
 def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0, align: int = 16,
@@ -145,7 +154,7 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
     rows = T * K + (align - 1) * El if max_rows is None else int(max_rows)
     if not 0 <= rows <= 1 << 30 or not -(1 << 31) <= local_expert_offset < (1 << 31):
         raise ValueError("max_rows or local_expert_offset out of range")
-    topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32)
+    topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32, (T, K))
     n = _sort_bytes(T, K, El, device)
     dev = topk_idx.device
     row0 = torch.empty(El + 1, dtype=_I32, device=dev)
@@ -159,23 +168,26 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
 
 def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, H] -> [max_rows, H]: row r is the row of its pair's token, zeros in the padding of a segment."""
-    kind, device = _rows_type(x, "x"), _device(x, "x")
+    x, x_at, kind, device, n, H = _rows(x, "x")
     row0, row_pair, pair_row, T, K, El, R = _order(order, device)
-    H = _hidden(x.shape[1])
-    x = _in(x, "x", device, x.dtype, (T, H), _ALIGN)
-    out, at = _out(out, "out", device, x[0], x[0].dtype, (R, H), _ALIGN, x, row0, row_pair, pair_row)
-    _call(_lib.lib.b200moe_permute, device, x[1], kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
+    if n != T:
+        _shape(x, "x", (T, H), x.dtype)
+    out, at = _out(out, "out", device, x, x.dtype, (R, H), _ALIGN, (x, x_at), row0, row_pair, pair_row)
+    _call(_lib.lib.b200moe_permute, device, x_at, kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
     return out
 
 
 def _combine(rows, w, order, out):
-    kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
+    rows, rows_at, kind, device, n, H = _rows(rows, "rows")
     row0, row_pair, pair_row, T, K, El, R = _order(order, device)
-    H = _hidden(rows.shape[1])
-    rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
-    w = (None, None) if w is None else _in(w, "topk_w", device, _F32, (T, K))
-    out, at = _out(out, "out", device, rows[0], rows[0].dtype, (T, H), _ALIGN, rows, pair_row, *((w,) if w[1] else ()))
-    _call(_lib.lib.b200moe_combine, device, rows[1], kind, w[1], pair_row[1], T, K, H, R, at)
+    if n != R:
+        _shape(rows, "rows", (R, H), rows.dtype)
+    inputs, w_at = ((rows, rows_at), pair_row), None
+    if w is not None:
+        w, w_at = _in(w, "topk_w", device, _F32, (T, K))
+        inputs += ((w, w_at),)
+    out, at = _out(out, "out", device, rows, rows.dtype, (T, H), _ALIGN, *inputs)
+    _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row[1], T, K, H, R, at)
     return out
 
 
@@ -193,15 +205,15 @@ def combine(rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Op
 
 def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None):
     """Gradients of `combine`: (grad_rows [max_rows, H], grad_w fp32 [T, top_k]); `out` takes the first."""
-    kind, device = _rows_type(rows, "rows"), _device(rows, "rows")
+    rows, rows_at, kind, device, n, H = _rows(rows, "rows")
     row0, row_pair, pair_row, T, K, El, R = _order(order, device)
-    H = _hidden(rows.shape[1])
-    rows = _in(rows, "rows", device, rows.dtype, (R, H), _ALIGN)
-    grad_out = _in(grad_out, "grad_out", device, rows[0].dtype, (T, H), _ALIGN)
+    if n != R:
+        _shape(rows, "rows", (R, H), rows.dtype)
+    grad_out = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
     topk_w = _in(topk_w, "topk_w", device, _F32, (T, K))
-    out, at = _out(out, "out", device, rows[0], rows[0].dtype, (R, H), _ALIGN, rows, grad_out, topk_w, row0, row_pair, pair_row)
+    out, at = _out(out, "out", device, rows, rows.dtype, (R, H), _ALIGN, (rows, rows_at), grad_out, topk_w, row0, row_pair, pair_row)
     grad_w = topk_w[0].new_empty((T, K))
-    _call(_lib.lib.b200moe_combine_backward, device, grad_out[1], rows[1], kind, topk_w[1], row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at,
+    _call(_lib.lib.b200moe_combine_backward, device, grad_out[1], rows_at, kind, topk_w[1], row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at,
           grad_w.data_ptr())
     return out, grad_w
 
@@ -214,13 +226,14 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
         raise ValueError("q must be e4m3 [T, H]")
     device = _device(q, "q")
     T, H = q.shape
-    _hidden(H)
+    if H <= 0 or H % 128 or H > 1 << 20:
+        raise ValueError(f"q: columns must be a multiple of 128 up to 2^20, got {H}")
     if out is not None:
         dtype = out.dtype
     kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"rows are bf16, fp16 or fp32, not {dtype}")
-    q = _in(q, "q", device, _E4M3, None, 16)
+    q = _in(q, "q", device, _E4M3, (T, H), 16)
     scale = _in(scale, "scale", device, _F32, (H // 128, T))
     if order is None:
         out, at = _out(out, "out", device, q[0], dtype, (T, H), _ALIGN, q, scale)
@@ -241,7 +254,7 @@ def _used(expert_row0, device):
     n = expert_row0.numel()
     if expert_row0.dim() != 1 or n < 1:
         raise ValueError("expert_row0 must be int32 [E_local + 1]")
-    t, at = _in(expert_row0, "expert_row0", device, _I32)
+    t, at = _in(expert_row0, "expert_row0", device, _I32, (n,))
     return t, at + 4 * (n - 1)
 
 
@@ -250,17 +263,13 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
     of its inputs for `swiglu_backward`.  A group of 128 columns is scaled by the smallest power of two not below its largest
     magnitude / 448; one that holds an infinity or a NaN gets the scale NaN.  `expert_row0`: only its last entry's number of rows is in use (None:
     all).  `out`: the three tensors to write."""
-    kind, device = _rows_type(gemm1_rows, "gemm1_rows"), _device(gemm1_rows, "gemm1_rows")
-    R, I2 = gemm1_rows.shape
-    if I2 <= 0 or I2 % 256 or I2 > 1 << 21:
-        raise ValueError(f"gemm1_rows must have 2 * I columns, I a multiple of 128 up to 2^20, got {I2}")
+    x, x_at, kind, device, R, I2 = _rows(gemm1_rows, "gemm1_rows", 256)
     keep, used = _used(expert_row0, device)
-    x = _in(gemm1_rows, "gemm1_rows", device, gemm1_rows.dtype, None, _ALIGN)
     act, q, scale = (None, None, None) if out is None else out
-    act = _out(act, "act", device, x[0], x[0].dtype, (R, I2 // 2), _ALIGN, x)
-    q = _out(q, "q", device, x[0], _E4M3, (R, I2), 16, x, act)
-    scale = _out(scale, "scale", device, x[0], _F32, (I2 // 128, R), 4, x, act, q)
-    _call(_lib.lib.b200moe_swiglu_save, device, x[1], kind, used, R, I2 // 2, act[1], q[1], scale[1])
+    act = _out(act, "act", device, x, x.dtype, (R, I2 // 2), _ALIGN, (x, x_at))
+    q = _out(q, "q", device, x, _E4M3, (R, I2), 16, (x, x_at), act)
+    scale = _out(scale, "scale", device, x, _F32, (I2 // 128, R), 4, (x, x_at), act, q)
+    _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act[1], q[1], scale[1])
     return act[0], q[0], scale[0]
 
 
@@ -268,20 +277,16 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
                     with_act: bool = True, out=None):
     """Gradient of `swiglu_save`'s activation from its 8-bit copy: (grad of gemm1_rows [R, 2I], act [R, I] again or None), both of
     grad_act's type.  `out`: the two tensors to write (the second None without `with_act`)."""
-    kind, device = _rows_type(grad_act, "grad_act"), _device(grad_act, "grad_act")
-    R, I = grad_act.shape
-    if I <= 0 or I % 128 or I > 1 << 20:
-        raise ValueError(f"grad_act must have I columns, a multiple of 128 up to 2^20, got {I}")
+    d, d_at, kind, device, R, I = _rows(grad_act, "grad_act")
     keep, used = _used(expert_row0, device)
     q = _in(q, "q", device, _E4M3, (R, 2 * I), 16)
     scale = _in(scale, "scale", device, _F32, (2 * I // 128, R))
-    d = _in(grad_act, "grad_act", device, grad_act.dtype, None, _ALIGN)
     grad_x, act = (None, None) if out is None else out
     if act is not None and not with_act:
         raise ValueError("out has a tensor for act, which with_act=False does not compute")
-    grad_x = _out(grad_x, "grad_gemm1_rows", device, d[0], d[0].dtype, (R, 2 * I), _ALIGN, q, scale, d)
-    act = _out(act, "act", device, d[0], d[0].dtype, (R, I), _ALIGN, q, scale, d, grad_x) if with_act else (None, None)
-    _call(_lib.lib.b200moe_swiglu_backward, device, q[1], scale[1], d[1], kind, used, R, I, grad_x[1], act[1])
+    grad_x = _out(grad_x, "grad_gemm1_rows", device, d, d.dtype, (R, 2 * I), _ALIGN, q, scale, (d, d_at))
+    act = _out(act, "act", device, d, d.dtype, (R, I), _ALIGN, q, scale, (d, d_at), grad_x) if with_act else (None, None)
+    _call(_lib.lib.b200moe_swiglu_backward, device, q[1], scale[1], d_at, kind, used, R, I, grad_x[1], act[1])
     return grad_x[0], act[0]
 
 
@@ -298,7 +303,7 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
     routing_mode = int(routing_mode)
     if not 0 <= routing_mode <= 5 or (routing_mode == 4 and K != 1):
         raise ValueError("routing_mode must be one of ROUTING_* (0 to 5; mode 4 picks one expert)")
-    logits = _in(routing_logits, "routing_logits", device, _F32, None, 16)
+    logits = _in(routing_logits, "routing_logits", device, _F32, (T, E), 16)
     bias = (None, None) if routing_bias is None else _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,))
     topk_idx = _in(topk_idx, "topk_idx", device, _I32, (T, K))
     grad_w = _in(grad_w, "grad_w", device, _F32, (T, K))
