@@ -12,7 +12,8 @@
 // token picks twice gets the sum of both; ids outside [0, E) carry no weight.
 // A token costs E floats written, zeros where nothing was picked, and a chain of dependent loads (pick, logit): a warp takes four
 // tokens, clears their rows - one run of memory - while the picks are on their way, and stores the picks' gradients behind that.
-// The default form reads the row whole, keeps it in registers and takes one token per warp.
+// The default form reads the row whole, keeps it in registers and takes one token per warp.  8192 tokens over 256 experts 2.7 us (one token per
+// warp, rows cleared first: 5.3), default 6.3; one token 1.6 and 2.0, which is the launch.
 #pragma once
 #include <cuda_bf16.h>
 #include "common.cuh"

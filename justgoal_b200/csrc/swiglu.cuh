@@ -11,6 +11,10 @@
 // nothing to amax / 448 but one of the 15 binades above its subnormals.  Under the scale 2^120 the codes end at 240, so that no finite value is
 // restored as an infinity (off by less than 2^-4, like any other code).  A group that holds an infinity or a NaN gets the scale NaN: its values
 // are gone, and the gradients made from it say so instead of being finite.
+// Byte work: 2048 columns of bf16, 34645 rows in use, save 91 us, backward with the activation 110 us in a row of such calls: 96 and 100 % of
+// the measured copy rate over the bytes that have to move; 8000 rows 24 and 28 us (83 and 89 %), 20000 rows of 256 columns 10 and 11 us.  The
+// save kernel issues in 64 % of its cycles (counters), so the arithmetic is kept short: products with powers of two instead of divisions, the
+// fast exponential for 16-bit rows.
 #pragma once
 #include "order.cuh"
 

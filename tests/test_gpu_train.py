@@ -72,7 +72,8 @@ def _order(T, K, El, seed, E=None, off=0):
 @pytest.mark.parametrize("T,K,E,El,off,align", [
     (0, 8, 64, 64, 0, 16), (1, 1, 32, 32, 0, 16), (1, 8, 256, 256, 0, 16), (7, 8, 256, 32, 96, 16), (33, 3, 64, 1, 5, 1), (128, 8, 64, 16, 16, 128),
     (511, 8, 256, 256, 0, 16), (512, 8, 512, 512, 0, 16), (513, 8, 96, 96, 0, 32), (1500, 5, 160, 40, 120, 2), (4097, 1, 32, 32, 0, 64),
-    (5000, 8, 512, 512, 0, 8), (14107, 8, 256, 256, 0, 16)])
+    (5000, 8, 512, 512, 0, 8), (14107, 8, 256, 256, 0, 16), (256, 8, 64, 64, 0, 16), (257, 8, 64, 64, 0, 16),
+    (160001, 8, 64, 64, 0, 16)])          # (slices of more than one chunk)
 def test_sort_tables(T, K, E, El, off, align):
     from justgoal_b200 import sort_tokens
     idx = _picks(T, K, E, seed=T + K, skew=0.7)
@@ -111,7 +112,9 @@ def test_sort_room_for_fewer_rows(T, max_rows):
 # ------------------------------------------------------------------ rows
 
 SIZES = [(1, 1, 32, 128, "bf16"), (5, 8, 32, 128, "fp16"), (37, 3, 64, 384, "fp32"), (200, 8, 32, 1152, "bf16"), (64, 8, 256, 7168, "bf16"),
-         (33, 8, 128, 4096, "fp16"), (301, 6, 96, 640, "fp32"), (3000, 2, 32, 256, "bf16"), (0, 8, 32, 256, "bf16")]
+         (33, 8, 128, 4096, "fp16"), (301, 6, 96, 640, "fp32"), (3000, 2, 32, 256, "bf16"), (0, 8, 32, 256, "bf16"),
+         # the combine's gradient by tokens with groups of 32 and 128 threads, by rows with 64, and either side of its line
+         (400, 8, 32, 256, "bf16"), (300, 8, 64, 7168, "bf16"), (20, 8, 32, 2048, "bf16"), (256, 7, 32, 512, "fp32"), (257, 7, 32, 512, "fp16")]
 
 
 def _rows(R, H, dtype, seed, device="cuda"):
@@ -218,6 +221,27 @@ def test_combine_backward(T, K, E, H, kind, share):
     dot[pair], mags[pair] = prod.sum(dim=1), prod.abs().sum(dim=1)
     assert grad_w.dtype == torch.float32 and grad_w.shape == (T, K)
     _check(grad_w, dot.view(T, K), (H / 32 + 13) * U * mags.view(T, K))
+
+
+@pytest.mark.parametrize("max_rows", [100, 333])
+def test_pairs_without_room_count_as_absent(max_rows):
+    """A capacity below the batch's rows: what does not fit has no row, adds nothing and gets no gradient."""
+    from justgoal_b200 import combine, combine_backward, permute, permute_backward, sort_tokens
+    T, K, H = 60, 6, 256
+    idx = _picks(T, K, 32, seed=31)
+    tables = oracle_order(idx, 32, max_rows=max_rows)
+    order = sort_tokens(idx.cuda(), 32, max_rows=max_rows)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(order, tables)) and bool((tables[2] < 0).any())
+    x, g, w = _rows(T, H, torch.float32, 1), _rows(T, H, torch.float32, 2), torch.rand(T, K, generator=_gen(5))
+    rows = permute(x, order)
+    live = tables[1] >= 0
+    assert torch.equal(rows.cpu()[live], x.cpu()[(tables[1][live] // K).long()])
+    want, mags = _combine64(rows.cpu(), w, tables, T)
+    _check(combine(rows, w.cuda(), order), want, K * U * mags)
+    grad_rows, grad_w = combine_backward(g, rows, w.cuda(), order)
+    assert bool((grad_w.cpu()[tables[2] < 0] == 0).all()) and bool((grad_w.cpu()[tables[2] >= 0] != 0).all())
+    want, mags = _combine64(grad_rows.cpu(), torch.ones(T, K), tables, T)
+    _check(permute_backward(grad_rows, order), want, K * U * mags)
 
 
 def test_order_without_local_pairs_and_without_room():
@@ -364,7 +388,7 @@ def _sigmoid_error(gate, dtype):
 
 
 SWIGLU = [(1, 128, "bf16"), (3, 128, "fp32"), (77, 256, "fp16"), (130, 1280, "bf16"), (9, 2048, "bf16"), (1000, 384, "fp16"), (257, 640, "fp32"),
-          (5, 8320, "bf16"), (4099, 128, "bf16")]
+          (5, 8320, "bf16"), (4099, 128, "bf16"), (20003, 256, "bf16")]
 
 
 @pytest.mark.parametrize("R,inner,kind", SWIGLU)
@@ -771,6 +795,30 @@ def test_a_step_of_training(T, E, El, off, keep8):
     for name, w in want.items():
         off_by = (got[name].double().cpu() - w).norm() / w.norm()
         assert float(off_by) <= 3.5e-3, (name, float(off_by))
+
+
+def test_wrapped_for_autograd():
+    """The pattern of the integration notes: the gradients of the explicit calls, bit for bit."""
+    import justgoal_b200 as jg
+
+    class Combine(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, rows, topk_w, order):
+            ctx.order = order
+            ctx.save_for_backward(rows, topk_w)
+            return jg.combine(rows, topk_w, order)
+
+        @staticmethod
+        def backward(ctx, grad_out):
+            return (*jg.combine_backward(grad_out, *ctx.saved_tensors, ctx.order), None)
+
+    order, tables = _order(50, 4, 32, seed=3)
+    used = int(tables[0][-1])
+    rows, w, g = _rows(tables[1].numel(), 256, torch.float32, 1), torch.rand(50, 4, device="cuda"), _rows(50, 256, torch.float32, 2)
+    a, b = rows.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    Combine.apply(a, b, order).backward(g)
+    grad_rows, grad_w = jg.combine_backward(g, rows, w, order)
+    assert torch.equal(a.grad[:used], grad_rows[:used]) and torch.equal(b.grad, grad_w)
 
 
 def test_streams_graphs_and_repeats():
