@@ -146,7 +146,7 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
         raise ValueError(f"topk_idx must be int32 [T, top_k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
     device = _device(topk_idx, "topk_idx")
     T, K = topk_idx.shape
-    El = int(num_local_experts)
+    El, align, local_expert_offset = int(num_local_experts), int(align), int(local_expert_offset)
     if not 1 <= K <= 8 or not 1 <= El <= 512 or T * K > 1 << 30:
         raise ValueError("1 to 8 picks per token, 1 to 512 local experts, at most 2^30 pairs")
     if align not in (1, 2, 4, 8, 16, 32, 64, 128):
