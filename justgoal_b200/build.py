@@ -38,7 +38,7 @@ def build(force: bool = False, verbose: bool = False, out: str = None) -> str:
     if out is None and not force and not needs_build():
         return LIB
     cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
-           "-shared", "-Xcompiler", "-fPIC", "--threads", "0", "-I", os.path.join(HERE, "..", "include"),
+           "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(HERE, "..", "include"),
            "-o", out or LIB] + [os.path.join(CSRC, s) for s in SOURCES]
     extra = os.environ.get("B200MOE_NVCC_FLAGS")      # e.g. -DB200MOE_ENABLE_KLOG for the per-K-block log
     if extra:

@@ -72,14 +72,14 @@ def _device(t, name):
     return device
 
 
-def _shape(t, name, shape, dtype):
+def _off(t, name, dtype, shape):
     raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _in(t, name, device, dtype, shape, align=1):
     """An input of a known form: (the tensor, its address); copied if it is not contiguous or not aligned."""
     if t.dtype is not dtype or t.shape != shape:
-        _shape(t, name, shape, dtype)
+        _off(t, name, dtype, shape)
     if t.get_device() != device:
         raise ValueError(f"{name} is not on cuda:{device}")
     at = t.data_ptr()
@@ -94,7 +94,9 @@ def _rows(t, name, columns=128):
     kind = _TYPES.get(t.dtype)
     if kind is None or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
-    device = _device(t, name)
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
     n, H = t.shape
     if H <= 0 or H % columns or H > columns << 13:
         raise ValueError(f"{name}: columns must be a multiple of {columns} up to {columns << 13}, got {H}")
@@ -105,35 +107,33 @@ def _rows(t, name, columns=128):
     return t, at, kind, device, n, H
 
 
-def _out(t, name, device, like, dtype, shape, align, *inputs):
-    """An output and its address: made here, or the caller's if it has the form that is written in place and shares no memory with the
-    inputs (tensor, address)."""
-    if t is None:
-        t = like.new_empty(shape, dtype=dtype)
-        return t, t.data_ptr()
+def _given(t, name, device, dtype, shape, align, *others):
+    """The address of the caller's output, which has to be of the form that is written in place and share no memory with the call's
+    rows and other outputs."""
     at = t.data_ptr()
     if t.dtype is not dtype or t.shape != shape or t.get_device() != device or at % align or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on cuda:{device} that starts at a multiple of {align} bytes")
     end = at + t.nbytes
-    for other, start in inputs:
+    for other in others:
+        start = other.data_ptr()
         if start < end and at < start + other.nbytes and at < end:
             raise ValueError(f"{name} must not share memory with an input or another output")
-    return t, at
+    return at
 
 
 def _order(order, device):
-    """An order's ((expert_row0, address), (row_pair, address), (pair_row, address), T, top_k, E_local, rows)."""
+    """An order's tables (kept by the caller until the call is made), their addresses, T, top_k, E_local, rows."""
     row0, row_pair, pair_row = order
     if not (row0.dtype is _I32 and row_pair.dtype is _I32 and pair_row.dtype is _I32 and row0.dim() == 1 and row_pair.dim() == 1
             and pair_row.dim() == 2 and row0.get_device() == device and row_pair.get_device() == device and pair_row.get_device() == device):
         raise ValueError(f"an order is int32 expert_row0 [E_local + 1], row_pair [max_rows] and pair_row [T, top_k] on cuda:{device}")
     if not (row0.is_contiguous() and row_pair.is_contiguous() and pair_row.is_contiguous()):
-        row0, row_pair, pair_row = row0.contiguous(), row_pair.contiguous(), pair_row.contiguous()
+        order = row0, row_pair, pair_row = row0.contiguous(), row_pair.contiguous(), pair_row.contiguous()
     T, K = pair_row.shape
     El = row0.numel() - 1
     if not (1 <= El <= 512 and 1 <= K <= 8):
         raise ValueError("an order has 1 to 512 local experts and 1 to 8 picks per token")
-    return (row0, row0.data_ptr()), (row_pair, row_pair.data_ptr()), (pair_row, pair_row.data_ptr()), T, K, El, row_pair.numel()
+    return order, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T, K, El, row_pair.numel()
 
 
 def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0, align: int = 16,
@@ -169,25 +169,30 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
 def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, H] -> [max_rows, H]: row r is the row of its pair's token, zeros in the padding of a segment."""
     x, x_at, kind, device, n, H = _rows(x, "x")
-    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    order, row0, row_pair, pair_row, T, K, El, R = _order(order, device)
     if n != T:
-        _shape(x, "x", (T, H), x.dtype)
-    out, at = _out(out, "out", device, x, x.dtype, (R, H), _ALIGN, (x, x_at), row0, row_pair, pair_row)
-    _call(_lib.lib.b200moe_permute, device, x_at, kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
+        _off(x, "x", x.dtype, (T, H))
+    if out is None:
+        out = x.new_empty((R, H))
+        at = out.data_ptr()
+    else:
+        at = _given(out, "out", device, x.dtype, (R, H), _ALIGN, x)
+    _call(_lib.lib.b200moe_permute, device, x_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
     return out
 
 
 def _combine(rows, w, order, out):
     rows, rows_at, kind, device, n, H = _rows(rows, "rows")
-    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    order, _, _, pair_row, T, K, _, R = _order(order, device)
     if n != R:
-        _shape(rows, "rows", (R, H), rows.dtype)
-    inputs, w_at = ((rows, rows_at), pair_row), None
-    if w is not None:
-        w, w_at = _in(w, "topk_w", device, _F32, (T, K))
-        inputs += ((w, w_at),)
-    out, at = _out(out, "out", device, rows, rows.dtype, (T, H), _ALIGN, *inputs)
-    _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row[1], T, K, H, R, at)
+        _off(rows, "rows", rows.dtype, (R, H))
+    w, w_at = (None, None) if w is None else _in(w, "topk_w", device, _F32, (T, K))
+    if out is None:
+        out = rows.new_empty((T, H))
+        at = out.data_ptr()
+    else:
+        at = _given(out, "out", device, rows.dtype, (T, H), _ALIGN, rows)
+    _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row, T, K, H, R, at)
     return out
 
 
@@ -206,15 +211,18 @@ def combine(rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Op
 def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = None):
     """Gradients of `combine`: (grad_rows [max_rows, H], grad_w fp32 [T, top_k]); `out` takes the first."""
     rows, rows_at, kind, device, n, H = _rows(rows, "rows")
-    row0, row_pair, pair_row, T, K, El, R = _order(order, device)
+    order, row0, row_pair, pair_row, T, K, El, R = _order(order, device)
     if n != R:
-        _shape(rows, "rows", (R, H), rows.dtype)
-    grad_out = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
-    topk_w = _in(topk_w, "topk_w", device, _F32, (T, K))
-    out, at = _out(out, "out", device, rows, rows.dtype, (R, H), _ALIGN, (rows, rows_at), grad_out, topk_w, row0, row_pair, pair_row)
-    grad_w = topk_w[0].new_empty((T, K))
-    _call(_lib.lib.b200moe_combine_backward, device, grad_out[1], rows_at, kind, topk_w[1], row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at,
-          grad_w.data_ptr())
+        _off(rows, "rows", rows.dtype, (R, H))
+    grad_out, grad_at = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
+    topk_w, w_at = _in(topk_w, "topk_w", device, _F32, (T, K))
+    if out is None:
+        out = torch.empty_like(rows)
+        at = out.data_ptr()
+    else:
+        at = _given(out, "out", device, rows.dtype, (R, H), _ALIGN, rows, grad_out)
+    grad_w = torch.empty_like(topk_w)
+    _call(_lib.lib.b200moe_combine_backward, device, grad_at, rows_at, kind, w_at, row0, row_pair, pair_row, T, K, El, H, R, at, grad_w.data_ptr())
     return out, grad_w
 
 
@@ -233,22 +241,26 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
     kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"rows are bf16, fp16 or fp32, not {dtype}")
-    q = _in(q, "q", device, _E4M3, (T, H), 16)
-    scale = _in(scale, "scale", device, _F32, (H // 128, T))
+    q, q_at = _in(q, "q", device, _E4M3, (T, H), 16)
+    scale, scale_at = _in(scale, "scale", device, _F32, (H // 128, T))
     if order is None:
-        out, at = _out(out, "out", device, q[0], dtype, (T, H), _ALIGN, q, scale)
-        _call(_lib.lib.b200moe_restore_1x128, device, q[1], scale[1], kind, None, None, None, T, 1, 1, H, T, at)
-        return out
-    row0, row_pair, pair_row, tokens, K, El, R = _order(order, device)
-    if tokens != T:
-        raise ValueError(f"q has {T} tokens, the order {tokens}")
-    out, at = _out(out, "out", device, q[0], dtype, (R, H), _ALIGN, q, scale, row0, row_pair, pair_row)
-    _call(_lib.lib.b200moe_restore_1x128, device, q[1], scale[1], kind, row0[1], row_pair[1], pair_row[1], T, K, El, H, R, at)
+        row0 = row_pair = pair_row = None
+        K, El, R = 1, 1, T
+    else:
+        order, row0, row_pair, pair_row, tokens, K, El, R = _order(order, device)
+        if tokens != T:
+            raise ValueError(f"q has {T} tokens, the order {tokens}")
+    if out is None:
+        out = q.new_empty((R, H), dtype=dtype)
+        at = out.data_ptr()
+    else:
+        at = _given(out, "out", device, dtype, (R, H), _ALIGN, q, scale)
+    _call(_lib.lib.b200moe_restore_1x128, device, q_at, scale_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
     return out
 
 
 def _used(expert_row0, device):
-    """(the table kept alive, address of its last entry: the number of rows in use)"""
+    """(the table, kept by the caller until the call is made; the address of its last entry: the number of rows in use)"""
     if expert_row0 is None:
         return None, None
     n = expert_row0.numel()
@@ -265,12 +277,17 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
     all).  `out`: the three tensors to write."""
     x, x_at, kind, device, R, I2 = _rows(gemm1_rows, "gemm1_rows", 256)
     keep, used = _used(expert_row0, device)
-    act, q, scale = (None, None, None) if out is None else out
-    act = _out(act, "act", device, x, x.dtype, (R, I2 // 2), _ALIGN, (x, x_at))
-    q = _out(q, "q", device, x, _E4M3, (R, I2), 16, (x, x_at), act)
-    scale = _out(scale, "scale", device, x, _F32, (I2 // 128, R), 4, (x, x_at), act, q)
-    _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act[1], q[1], scale[1])
-    return act[0], q[0], scale[0]
+    if out is None:
+        act, q = x.new_empty((R, I2 // 2)), x.new_empty((R, I2), dtype=_E4M3)
+        scale = x.new_empty((I2 // 128, R), dtype=_F32)
+        act_at, q_at, scale_at = act.data_ptr(), q.data_ptr(), scale.data_ptr()
+    else:
+        act, q, scale = out
+        act_at = _given(act, "act", device, x.dtype, (R, I2 // 2), _ALIGN, x)
+        q_at = _given(q, "q", device, _E4M3, (R, I2), 16, x, act)
+        scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), 4, x, act, q)
+    _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act_at, q_at, scale_at)
+    return act, q, scale
 
 
 def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor, expert_row0: Optional[torch.Tensor] = None,
@@ -279,15 +296,19 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
     grad_act's type.  `out`: the two tensors to write (the second None without `with_act`)."""
     d, d_at, kind, device, R, I = _rows(grad_act, "grad_act")
     keep, used = _used(expert_row0, device)
-    q = _in(q, "q", device, _E4M3, (R, 2 * I), 16)
-    scale = _in(scale, "scale", device, _F32, (2 * I // 128, R))
-    grad_x, act = (None, None) if out is None else out
-    if act is not None and not with_act:
-        raise ValueError("out has a tensor for act, which with_act=False does not compute")
-    grad_x = _out(grad_x, "grad_gemm1_rows", device, d, d.dtype, (R, 2 * I), _ALIGN, q, scale, (d, d_at))
-    act = _out(act, "act", device, d, d.dtype, (R, I), _ALIGN, q, scale, (d, d_at), grad_x) if with_act else (None, None)
-    _call(_lib.lib.b200moe_swiglu_backward, device, q[1], scale[1], d_at, kind, used, R, I, grad_x[1], act[1])
-    return grad_x[0], act[0]
+    q, q_at = _in(q, "q", device, _E4M3, (R, 2 * I), 16)
+    scale, scale_at = _in(scale, "scale", device, _F32, (2 * I // 128, R))
+    if out is None:
+        grad_x, act = d.new_empty((R, 2 * I)), torch.empty_like(d) if with_act else None
+        grad_at, act_at = grad_x.data_ptr(), act.data_ptr() if with_act else None
+    else:
+        grad_x, act = out
+        if (act is not None) != with_act:
+            raise ValueError("out has a tensor for act if and only if with_act asks for it")
+        grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), _ALIGN, q, scale, d)
+        act_at = _given(act, "act", device, d.dtype, (R, I), _ALIGN, q, scale, d, grad_x) if with_act else None
+    _call(_lib.lib.b200moe_swiglu_backward, device, q_at, scale_at, d_at, kind, used, R, I, grad_at, act_at)
+    return grad_x, act
 
 
 def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Tensor], topk_idx: torch.Tensor, grad_w: torch.Tensor,
@@ -303,10 +324,14 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
     routing_mode = int(routing_mode)
     if not 0 <= routing_mode <= 5 or (routing_mode == 4 and K != 1):
         raise ValueError("routing_mode must be one of ROUTING_* (0 to 5; mode 4 picks one expert)")
-    logits = _in(routing_logits, "routing_logits", device, _F32, (T, E), 16)
-    bias = (None, None) if routing_bias is None else _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,))
-    topk_idx = _in(topk_idx, "topk_idx", device, _I32, (T, K))
-    grad_w = _in(grad_w, "grad_w", device, _F32, (T, K))
-    out, at = _out(out, "out", device, logits[0], _F32, (T, E), 16, logits, topk_idx, grad_w, *((bias,) if bias[1] else ()))
-    _call(_lib.lib.b200moe_route_backward, device, logits[1], bias[1], topk_idx[1], grad_w[1], T, E, K, float(routed_scaling_factor), routing_mode, at)
+    logits, logits_at = _in(routing_logits, "routing_logits", device, _F32, (T, E), 16)
+    bias, bias_at = (None, None) if routing_bias is None else _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,))
+    topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32, (T, K))
+    grad_w, grad_at = _in(grad_w, "grad_w", device, _F32, (T, K))
+    if out is None:
+        out = torch.empty_like(logits)
+        at = out.data_ptr()
+    else:
+        at = _given(out, "out", device, _F32, (T, E), 16, logits, grad_w)
+    _call(_lib.lib.b200moe_route_backward, device, logits_at, bias_at, idx_at, grad_at, T, E, K, float(routed_scaling_factor), routing_mode, at)
     return out
