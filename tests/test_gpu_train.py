@@ -888,3 +888,32 @@ def test_rows_past_32_bits():
     assert torch.equal(rows[R - 1], x[0]) and torch.equal(rows[0], x[0]) and torch.equal(rows[R - 2], x[1]) and torch.equal(rows[150001], x[1])
     out = combine(rows, torch.tensor([[1.0, 1.0], [0.5, 0.0]], device="cuda"), order)
     assert torch.equal(out[0], (2 * x[0].float()).to(torch.bfloat16)) and torch.equal(out[1], (0.5 * x[1].float()).to(torch.bfloat16))
+
+
+def test_swiglu_and_gradients_past_32_bits():
+    """More than 2^31 elements in a row buffer: the last rows' activation, 8-bit copy and gradients are those of the same rows alone."""
+    from justgoal_b200 import TokenOrder, combine_backward, swiglu_backward, swiglu_save
+    R, inner, n = 270000, 4096, 5
+    x = torch.zeros(R, 2 * inner, dtype=torch.bfloat16, device="cuda")
+    x[-n:] = _rows(n, 2 * inner, torch.bfloat16, 1)
+    act, q, scale = swiglu_save(x)
+    small = swiglu_save(x[-n:].clone())
+    assert torch.equal(act[-n:], small[0]) and torch.equal(q[-n:].view(torch.uint8), small[1].view(torch.uint8)) and torch.equal(scale[:, -n:], small[2])
+    assert not bool(act[:7].any()) and bool((scale[:, :7] == 1).all())
+    d = torch.zeros(R, inner, dtype=torch.bfloat16, device="cuda")
+    d[-n:] = _rows(n, inner, torch.bfloat16, 2)
+    grad, again = swiglu_backward(q, scale, d)
+    want = swiglu_backward(*small[1:], d[-n:].clone())
+    assert torch.equal(grad[-n:], want[0]) and torch.equal(again[-n:], want[1]) and not bool(grad[:7].any())
+    del act, q, scale, d, again
+    pair_row = torch.tensor([[R - 1, 3]], dtype=torch.int32, device="cuda")
+    row_pair = torch.full((R,), -1, dtype=torch.int32, device="cuda")
+    row_pair[R - 1], row_pair[3] = 0, 1
+    order = TokenOrder(torch.tensor([0, R], dtype=torch.int32, device="cuda"), row_pair, pair_row)
+    g, w = _rows(1, 2 * inner, torch.bfloat16, 3), torch.tensor([[0.5, 2.0]], device="cuda")
+    grad.fill_(7.0)
+    _, grad_w = combine_backward(g, x, w, order, out=grad)
+    assert torch.equal(grad[R - 1], (0.5 * g[0].float()).to(torch.bfloat16)) and torch.equal(grad[3], (2 * g[0].float()).to(torch.bfloat16))
+    assert not bool(grad[R - 2].any()) and not bool(grad[2].any()) and float(grad_w[0, 1]) == 0.0
+    dot = (g[0].double() * x[R - 1].double()).sum()
+    assert abs(float(grad_w[0, 0]) - float(dot)) <= (2 * inner / 32 + 13) * U * float((g[0].double() * x[R - 1].double()).abs().sum())
