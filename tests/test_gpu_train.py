@@ -316,6 +316,20 @@ def test_views_and_odd_starts_are_copied(kind):
             assert torch.equal(a, b)
 
 
+def test_broadcast_gradients():
+    """Gradients as a sum's backward pass gives them: one value, expanded."""
+    from justgoal_b200 import combine_backward, permute_backward, swiglu_backward, swiglu_save
+    order, tables = _order(30, 4, 32, seed=12)
+    used, R, H = int(tables[0][-1]), tables[1].numel(), 256
+    rows, w, one = _rows(R, H, torch.float32, 1), torch.rand(30, 4, device="cuda"), torch.full((1, 1), 0.5, device="cuda")
+    for a, b in zip(combine_backward(one.expand(30, H), rows, w, order), combine_backward(one.repeat(30, H), rows, w, order)):
+        assert torch.equal(a[:used], b[:used])
+    assert torch.equal(permute_backward(one.expand(R, H), order), permute_backward(one.repeat(R, H), order))
+    _, q, scale = swiglu_save(rows)
+    for a, b in zip(swiglu_backward(q, scale, one.expand(R, H // 2)), swiglu_backward(q, scale, one.repeat(R, H // 2))):
+        assert torch.equal(a, b)
+
+
 def test_outputs_that_cannot_be_written_are_refused():
     from justgoal_b200 import TokenOrder, combine, combine_backward, permute, restore_1x128, route_backward, swiglu_backward, swiglu_save
     order, tables = _order(8, 4, 32, seed=9)
