@@ -11,12 +11,12 @@
 // nothing to amax / 448 but one of the 15 binades above its subnormals.  Under the scale 2^120 the codes end at 240, so that no finite value is
 // restored as an infinity (off by less than 2^-4, like any other code).  A group that holds an infinity or a NaN gets the scale NaN: its values
 // are gone, and the gradients made from it say so instead of being finite.
-// Byte work: 2048 columns of bf16, 34645 rows in use, save 89 us, backward with the activation 110 us in a row of such calls: 98 and 100 % of
-// the measured copy rate over the bytes that have to move; 8000 rows 23 and 27 us (87 and 93 %), 20000 rows of 256 columns 9.6 and 10 us.  The
+// Byte work: 2048 columns of bf16, 34645 rows in use, save 88 us, backward with the activation 105 us in a row of such calls: 100 and 104 % of
+// the measured copy rate over the bytes that have to move; 8000 rows 23 and 26 us (87 and 96 %), 20000 rows of 256 columns 9.6 and 10 us.  The
 // arithmetic has to stay out of the way, also at the clocks of a long run under the power limit: products with powers of two instead of
 // divisions, two values per instruction, magnitudes compared two 16-bit patterns at a time, flushed approximations for 16-bit rows, no division in
 // the walk over a block.  With one value per instruction and the library's exponential and quotient the save kernel issued in 64 % of its cycles: 91 and
-// 110 us for short, 97 and 115 after a second of load (94 and 110 now), 2000 rows backward 10.0 us (8.6 now).
+// 110 us for short, 97 and 115 after a second of load (93 and 108 now).
 #pragma once
 #include "order.cuh"
 

@@ -92,18 +92,22 @@ int restore_rows(const OrderParams& o, const void* q, const float* scale, void* 
     return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
 }
 
-// Block of a CTA of the SwiGLU kernels: the fewest rows, four or eight at least, that keep the CTA's threads busy in nearly all of its turns (40000 x
-// 640, five groups: eight rows 44.3 us, 16: 39.4), fewer where that leaves less than two CTAs per SM.  Eight / four rows where both do
-// (2048 columns; save, backward): 2000 rows 9.7 / 7.4 us, 10.7 / 10.0, 8000: 25.1 / 24.3, 30.0 / 28.4, 34645: 90.9 / 90.7, 109.7 / 111.6;
-// so eight from 16 CTAs per SM on.
-void swiglu_block(int rows, int I, int& rsh, int& gpc, dim3& grid) {
+// Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; fewer rows where that leaves less than two CTAs per SM.
+// save: the fewest rows, four at least (half a sector of scales), that keep the CTA's threads busy in four fifths of its turns.  Two / four / eight rows
+// of 2048 columns, us: 2000 rows 7.4 / 7.2 / 9.2, 8000: 24.4 / 23.6 / 24.3, 34645: 93.8 / 88.6 / 89.8; eight / 16 / 32 of 640 columns (five groups: 62, 83
+// and 100 %) 40000 rows 42.0 / 38.0 / 38.8.
+// backward: nothing is kept between turns, so about one turn: two / four / eight rows of 2048 columns 8000 rows 26.7 / 27.4 / 28.2, 34645: 106.0 / 108.3 /
+// 110.6; four / eight / 16 of 640 columns 40.0 / 41.2 / 42.2; eight / 16 of 256 columns 20000 rows 10.1 / 10.2.
+void swiglu_block(bool save, int rows, int I, int& rsh, int& gpc, dim3& grid) {
     const int groups = I >> 7, parts = (groups + 63) / 64;
     gpc = (groups + parts - 1) / parts;
-    rsh = ((long long)rows >> 3) * parts >= 16ll * sm_count() ? 3 : 2;
-    while (rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES) {
-        const int items = gpc << rsh, turns = (items + SWIGLU_TURN - 1) / SWIGLU_TURN;
-        if (items * 10 >= turns * SWIGLU_TURN * 9) break;
-        ++rsh;
+    if (save) {
+        for (rsh = 2; rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES; ++rsh) {
+            const int items = gpc << rsh, turns = (items + SWIGLU_TURN - 1) / SWIGLU_TURN;
+            if (items * 5 >= turns * SWIGLU_TURN * 4) break;
+        }
+    } else {
+        for (rsh = 0; rsh < 5 && (gpc << rsh) * 8 < SWIGLU_TURN * 5; ++rsh) {}
     }
     while (rsh > 0 && (long long)((rows + (1 << rsh) - 1) >> rsh) * parts < 2ll * sm_count()) --rsh;
     grid = dim3((rows + (1 << rsh) - 1) >> rsh, (groups + gpc - 1) / gpc);
@@ -113,7 +117,7 @@ template <typename T>
 int swiglu_save(const void* x, const int32_t* used, int rows, int I, void* act, void* q, float* scale, void* stream) {
     int rsh, gpc;
     dim3 grid;
-    swiglu_block(rows, I, rsh, gpc, grid);
+    swiglu_block(true, rows, I, rsh, gpc, grid);
     return launch(swiglu_save_kernel<T>, grid, SWIGLU_THREADS, stream, static_cast<const T*>(x), used, rows, I, rsh, gpc, static_cast<T*>(act),
                   static_cast<uint8_t*>(q), scale);
 }
@@ -122,7 +126,7 @@ template <typename T>
 int swiglu_grad(const void* q, const float* scale, const void* d_act, const int32_t* used, int rows, int I, void* d_x, void* act, void* stream) {
     int rsh, gpc;
     dim3 grid;
-    swiglu_block(rows, I, rsh, gpc, grid);
+    swiglu_block(false, rows, I, rsh, gpc, grid);
     return launch(act ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>, grid, SWIGLU_THREADS, stream, static_cast<const uint8_t*>(q), scale,
                   static_cast<const T*>(d_act), used, rows, I, rsh, gpc, static_cast<T*>(d_x), static_cast<T*>(act));
 }
