@@ -271,8 +271,8 @@ struct OrderParams {
 };
 
 // Byte work, bound by HBM: at 7168 bf16 columns and 8 rows per token, 256 experts, permute 8192 tokens 168 us (6.5 TB/s of what it cannot do
-// without, 99 % of the copy rate measured on the same kind of card), restore 4096: 83 us (97 %), combine 4096: 79 us (102 %), its gradient 166 us
-// (95 %).  Every row crosses memory once (counters: bytes read and written within 1 % of the operands'), nothing is staged in shared memory:
+// without, 99 % of the copy rate measured on the same kind of card), restore 4096: 83 us (97 %), combine 4096: 79 us (102 %), its gradient 164 us
+// (96 %).  Every row crosses memory once (counters: bytes read and written within 1 % of the operands'), nothing is staged in shared memory:
 // the rows of a token are independent streams, and loads in flight are what fills the bus.  A warp per token (the first form) left lanes and steps
 // of a row empty and paid the look-up of its rows once per token: 183, 105, 91 and 166 us.
 //
@@ -503,15 +503,15 @@ __device__ __forceinline__ float grad_unit(const float* g, const uint4& row, flo
 // By tokens: a group of threads (whole warps) takes a token with all of its rows, so that d_out is read once and eight rows' loads are in
 // flight.  By rows: a group takes a row, with FLIGHT units of it in flight per thread, whichever token it belongs to; d_out comes from L2
 // as often as it has rows.
-constexpr int GRAD_FLIGHT = 4;
+constexpr int GRAD_FLIGHT = 4, GRAD_THREADS = 128, GRAD_WARPS = GRAD_THREADS / 32;
 template <typename T>
 __device__ __forceinline__ void combine_grad_by_rows(const OrderParams& o, const T* __restrict__ d_out, const T* __restrict__ rows, const float* __restrict__ w,
-                                                     T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, int used, float (*s_dot)[8][ORDER_MAX_PICKS]) {
+                                                     T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, int used, float (*s_dot)[GRAD_WARPS][ORDER_MAX_PICKS]) {
     constexpr int V = 16 / sizeof(T), FLIGHT = GRAD_FLIGHT;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const int groups = 256 >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
+    const int groups = GRAD_THREADS >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
     const int units = H / V, pairs = o.T * o.top_k;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pairs; i += gridDim.x * 256ll) {
+    for (long long i = blockIdx.x * (long long)GRAD_THREADS + threadIdx.x; i < pairs; i += gridDim.x * (long long)GRAD_THREADS) {
         const int r = __ldg(o.pair_row + i);
         if (r < 0 || r >= o.num_rows) d_w[i] = 0.f;
     }
@@ -561,10 +561,10 @@ __device__ __forceinline__ void combine_grad_by_rows(const OrderParams& o, const
 
 template <typename T>
 __device__ __forceinline__ void combine_grad_by_tokens(const OrderParams& o, const T* __restrict__ d_out, const T* __restrict__ rows, const float* __restrict__ w,
-                                                       T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, float (*s_dot)[8][ORDER_MAX_PICKS]) {
+                                                       T* __restrict__ d_rows, float* __restrict__ d_w, int H, int gsh, float (*s_dot)[GRAD_WARPS][ORDER_MAX_PICKS]) {
     constexpr int V = 16 / sizeof(T), K = ORDER_MAX_PICKS;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const int group = threadIdx.x >> gsh, groups = 256 >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
+    const int group = threadIdx.x >> gsh, groups = GRAD_THREADS >> gsh, stride = 1 << gsh, in = threadIdx.x & (stride - 1);
     const int units = H / V;
     int buf = 0;
     for (long long t0 = (long long)blockIdx.x * groups; t0 < o.T; t0 += (long long)gridDim.x * groups, buf ^= 1) {
@@ -606,15 +606,16 @@ __device__ __forceinline__ void combine_grad_by_tokens(const OrderParams& o, con
 
 // By rows for few tokens, and where few of the picks have a row here (an expert-parallel rank's share).  By tokens / by rows, us, 7168
 // columns: one token 9.6 / 3.2, 64: 16 / 17, 256: 24 / 24, 512: 32 / 34, 2048: 90 / 97, 4096: 166 / 196, 8192: 322 / 409; 4096 tokens with one row each 61 /
-// 30, two 72 / 53, four 99 / 98.  Groups of 2^row_sh or 2^token_sh threads.
+// 30, two 72 / 53, four 99 / 98 (CTAs of 256 threads).  Groups of 2^row_sh or 2^token_sh threads; with 256 threads per CTA, two tokens that wait for
+// each other in every turn, 512 tokens took 33.8 us (31.1 with 128), 4096: 165.9 (164.4).
 // In both ways all threads of a CTA make the same number of turns, as they meet in each; the sums' two buffers let a warp be one turn
 // ahead of the thread that reads them.
 constexpr int GRAD_FEW_TOKENS = 256, GRAD_FEW_ROWS = 3;
 template <typename T>
-__global__ void __launch_bounds__(256, 2) combine_grad_kernel(const OrderParams o, const T* __restrict__ d_out, const T* __restrict__ rows,
+__global__ void __launch_bounds__(GRAD_THREADS, 4) combine_grad_kernel(const OrderParams o, const T* __restrict__ d_out, const T* __restrict__ rows,
                                                               const float* __restrict__ w, T* __restrict__ d_rows, float* __restrict__ d_w, int H,
                                                               int token_sh, int row_sh) {
-    __shared__ float s_dot[2][8][ORDER_MAX_PICKS];
+    __shared__ float s_dot[2][GRAD_WARPS][ORDER_MAX_PICKS];
     pdl_wait();
     const int used = min(__ldg(o.expert_row0 + o.num_local), o.num_rows);
     if (o.T <= GRAD_FEW_TOKENS || used <= (long long)GRAD_FEW_ROWS * o.T) {

@@ -60,11 +60,11 @@ int check_order(const OrderParams& o, int H) {
 }
 
 // CTAs that look through the padding of `rows` rows: a row a warp, as long as the chip holds them at once
-long long padding_ctas(long long rows, int per_sm) { return min((rows + 7) / 8, (long long)per_sm * sm_count()); }
+long long padding_ctas(long long rows, int warps, int per_sm) { return min((rows + warps - 1) / warps, (long long)per_sm * sm_count()); }
 
 // Grid of a kernel whose threads take one unit of a token's row each
 int unit_grid(long long T, int units, long long pad_rows) {
-    return (int)min(max(max((T * units + 255) / 256, padding_ctas(pad_rows, 6)), 1ll), 1ll << 24);
+    return (int)min(max(max((T * units + 255) / 256, padding_ctas(pad_rows, 8, 6)), 1ll), 1ll << 24);
 }
 
 template <typename T>
@@ -81,9 +81,9 @@ int combine_grad(const OrderParams& o, const void* d_out, const void* rows, cons
     int token_sh = 5, row_sh = 5;
     while (token_sh < 7 && units > 4 << token_sh) ++token_sh;
     while (o.T <= 64 && row_sh < 7 && units >= 2 * GRAD_FLIGHT << row_sh) ++row_sh;
-    const long long ctas = ((long long)o.T + (256 >> token_sh) - 1) / (256 >> token_sh);
-    const int grid = (int)max(max(min(ctas, 8ll * sm_count()), padding_ctas(o.num_rows, 2)), 1ll);
-    return launch(combine_grad_kernel<T>, dim3(grid), 256, stream, o, static_cast<const T*>(d_out), static_cast<const T*>(rows), w,
+    const int tokens = GRAD_THREADS >> token_sh;
+    const int grid = (int)max(max(min(((long long)o.T + tokens - 1) / tokens, 16ll * sm_count()), padding_ctas(o.num_rows, GRAD_WARPS, 4)), 1ll);
+    return launch(combine_grad_kernel<T>, dim3(grid), GRAD_THREADS, stream, o, static_cast<const T*>(d_out), static_cast<const T*>(rows), w,
                   static_cast<T*>(d_rows), d_w, H, token_sh, row_sh);
 }
 
