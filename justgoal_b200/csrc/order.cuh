@@ -330,9 +330,11 @@ struct Padding {
     }
 };
 
-// rows[r] = x[t] for the token's rows: a unit is read once and stored up to top_k times.  (Few tokens are bound by the padding that they
-// make: 64 tokens over 256 experts write 55 MB of zeros beside 7 MB of rows, 11 us.)
-__global__ void __launch_bounds__(256) permute_rows_kernel(const OrderParams o, const char* __restrict__ x, char* __restrict__ rows, int units) {
+// rows[r] = x[t] for the token's rows: a unit is read once and stored up to top_k times.  Nothing is shared inside a CTA, and small ones start and
+// end evenly: 256 / 128 / 64 threads, 1 token 4.0 / 2.8 / 2.7 us, 64: 11.8 / 10.2 / 8.6 (55 MB of padding's zeros beside 7 MB of rows), 8192 tokens of
+// 128 columns 5.5 / 4.9 / 4.8, long calls of wide rows level.
+constexpr int PERMUTE_THREADS = 64;
+__global__ void __launch_bounds__(PERMUTE_THREADS) permute_rows_kernel(const OrderParams o, const char* __restrict__ x, char* __restrict__ rows, int units) {
     pdl_wait();
     Padding pad;
     pad.begin(o);
@@ -363,7 +365,7 @@ __device__ __forceinline__ void restore16(const uint4& q, float s, float* v) {
 
 // rows[r] = q[t] * scale, like permute_rows_kernel with units of 16 columns.  Without an order (pair_row null) row t is token t.
 template <typename T>
-__global__ void __launch_bounds__(256) restore_rows_kernel(const OrderParams o, const uint8_t* __restrict__ q, const float* __restrict__ scale,
+__global__ void __launch_bounds__(PERMUTE_THREADS) restore_rows_kernel(const OrderParams o, const uint8_t* __restrict__ q, const float* __restrict__ scale,
                                                            T* __restrict__ rows, int H) {
     pdl_wait();
     const bool ordered = o.pair_row != nullptr;
@@ -394,12 +396,13 @@ __global__ void __launch_bounds__(256) restore_rows_kernel(const OrderParams o, 
 
 // ---------------------------------------------------------------- rows back to their tokens
 // out[t] = sum_k w[t, k] rows[r(t, k)], w null: ones.  A thread takes 32-byte units, one after the other: while the rows of one are on their
-// way it looks up the rows of the next, so that the chain of dependent loads is paid once; up to eight rows' loads are in flight, which two
-// CTAs of 256 threads per SM leave registers for.  4096 tokens of 7168 columns: all eight rows here 79 us, half of them 47, an eighth 30 (a
+// way it looks up the rows of the next, so that the chain of dependent loads is paid once; up to eight rows' loads are in flight, which four
+// CTAs of 128 threads per SM leave registers for (two of 256: 1 token 2.1 us against 1.9, 1500 tokens 6.5 against 6.2).  4096 tokens of 7168 columns: all eight rows here 79 us, half of them 47, an eighth 30 (a
 // floor of 18: a thread then has one load in flight, but three or four CTAs with fewer loads each took 28 to 29 and cost the full case 8 us, and a
 // warp per token with four units in flight 33).
+constexpr int COMBINE_THREADS = 128, COMBINE_CTAS = 4;         // CTAs of an SM
 template <typename T>
-__global__ void __launch_bounds__(256, 2) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
+__global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_CTAS) combine_rows_kernel(const OrderParams o, const T* __restrict__ rows, const float* __restrict__ w,
                                                               T* __restrict__ out, int H) {
     constexpr int V = 32 / sizeof(T), K = ORDER_MAX_PICKS;
     pdl_wait();

@@ -64,14 +64,15 @@ long long padding_ctas(long long rows, int warps, int per_sm) { return min((rows
 
 // Grid of a kernel whose threads take one unit of a token's row each
 int unit_grid(long long T, int units, long long pad_rows) {
-    return (int)min(max(max((T * units + 255) / 256, padding_ctas(pad_rows, 8, 6)), 1ll), 1ll << 24);
+    return (int)min(max(max((T * units + PERMUTE_THREADS - 1) / PERMUTE_THREADS, padding_ctas(pad_rows, PERMUTE_THREADS / 32, 1536 / PERMUTE_THREADS)), 1ll),
+                    1ll << 24);
 }
 
 template <typename T>
 int combine_rows(const OrderParams& o, const void* rows, const float* w, void* out, int H, void* stream) {
     const long long units = (long long)o.T * (H * (int)sizeof(T) / 32);
-    const int grid = (int)min((units + 255) / 256, 2ll * sm_count());
-    return launch(combine_rows_kernel<T>, dim3(grid), 256, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
+    const int grid = (int)min((units + COMBINE_THREADS - 1) / COMBINE_THREADS, (long long)COMBINE_CTAS * sm_count());
+    return launch(combine_rows_kernel<T>, dim3(grid), COMBINE_THREADS, stream, o, static_cast<const T*>(rows), w, static_cast<T*>(out), H);
 }
 
 template <typename T>
@@ -89,7 +90,8 @@ int combine_grad(const OrderParams& o, const void* d_out, const void* rows, cons
 
 template <typename T>
 int restore_rows(const OrderParams& o, const void* q, const float* scale, void* rows, int H, void* stream) {
-    return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), 256, stream, o, static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
+    return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), PERMUTE_THREADS, stream, o,
+                  static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
 }
 
 // Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; fewer rows where that leaves less than two CTAs per SM.
@@ -167,7 +169,7 @@ int b200moe_permute(const void* x, int type, const int32_t* expert_row0, const i
     if (num_rows == 0) return 0;
     if (!expert_row0 || !row_pair || !rows || (T && (!x || !pair_row)) || misaligned(x, 32) || misaligned(rows, 32)) return B200MOE_E_BADARG;
     const int units = hidden * type_bytes(type) / 32;
-    return launch(permute_rows_kernel, unit_grid(T, units, num_rows), 256, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
+    return launch(permute_rows_kernel, unit_grid(T, units, num_rows), PERMUTE_THREADS, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
 }
 
 int b200moe_restore_1x128(const void* q, const float* scale, int type, const int32_t* expert_row0, const int32_t* row_pair, const int32_t* pair_row,
