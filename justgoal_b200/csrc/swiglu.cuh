@@ -12,18 +12,19 @@
 // restored as an infinity (off by less than 2^-4, like any other code).  A group that holds an infinity or a NaN gets the scale NaN: its values
 // are gone, and the gradients made from it say so instead of being finite.
 // Byte work: 2048 columns of bf16, 34645 rows in use, save 88 us, backward with the activation 105 us in a row of such calls: 100 and 104 % of
-// the measured copy rate over the bytes that have to move; 8000 rows 23 and 26 us (87 and 96 %), 20000 rows of 256 columns 9.6 and 10 us.  The
+// the measured copy rate over the bytes that have to move; 8000 rows 23 and 26 us (88 and 96 %), 20000 rows of 256 columns 9.2 and 10 us.  The
 // arithmetic has to stay out of the way, also at the clocks of a long run under the power limit: products with powers of two instead of
 // divisions, two values per instruction, magnitudes compared two 16-bit patterns at a time, flushed approximations for 16-bit rows, no division in
 // the walk over a block.  With one value per instruction and the library's exponential and quotient the save kernel issued in 64 % of its cycles: 91 and
-// 110 us for short, 97 and 115 after a second of load (93 and 108 now).
+// 110 us for short, 97 and 115 after a second of load (92 and 108 now).
 #pragma once
 #include "order.cuh"
 
 namespace b200moe {
 
-constexpr int SWIGLU_THREADS = 256, SWIGLU_LANES = 8;        // lanes of a group of 128 columns, 16 each
-constexpr int SWIGLU_TURN = SWIGLU_THREADS / SWIGLU_LANES;   // pairs of groups a CTA takes at a time
+constexpr int SWIGLU_LANES = 8;                                        // lanes of a group of 128 columns, 16 each
+constexpr int SAVE_THREADS = 128, SAVE_TURN = SAVE_THREADS / SWIGLU_LANES;       // pairs of groups a CTA takes at a time
+constexpr int GRAD_X_THREADS = 256, GRAD_X_TURN = GRAD_X_THREADS / SWIGLU_LANES;
 constexpr int SWIGLU_SCALES = 512;                           // most pairs of groups of a CTA
 
 // Two sigmoids, 1 / (1 + 2^(-g log2 e)).  16-bit rows take the fast exponential and reciprocal, flushed: off by a few units of 2^-23, and zero for
@@ -138,13 +139,14 @@ __device__ __forceinline__ float2 decode2(const uint4& q, int i, float s) {
     return __fmul2_rn(e4m3x2_to_f32x2((uint16_t)(i & 1 ? w >> 16 : w)), make_float2(s, s));
 }
 
-// The eight lanes' next (row, group) of a CTA's block without a division per step
+// The eight lanes' next (row, group) of a CTA's block, TURN of them further on, without a division per step
+template <int TURN>
 struct BlockWalk {
     int r, j, dr, dj, nj;
     __device__ __forceinline__ BlockWalk(int nj_) : nj(nj_) {
         const int i = threadIdx.x >> 3;
         r = i / nj; j = i - r * nj;
-        dr = SWIGLU_TURN / nj; dj = SWIGLU_TURN - dr * nj;
+        dr = TURN / nj; dj = TURN - dr * nj;
     }
     __device__ __forceinline__ void step() {
         r += dr; j += dj;
@@ -156,7 +158,7 @@ struct BlockWalk {
 // group j of up and of gate, 32 bytes (16-bit types) of each per lane; scales wait in shared memory until a group's run of rows
 // leaves as one store.
 template <typename T>
-__global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_save_kernel(const T* __restrict__ x, const int32_t* __restrict__ used, int rows, int I, int rsh,
+__global__ void __launch_bounds__(SAVE_THREADS) swiglu_save_kernel(const T* __restrict__ x, const int32_t* __restrict__ used, int rows, int I, int rsh,
                                                                      int gpc, T* __restrict__ act, uint8_t* __restrict__ q, float* __restrict__ scale) {
     __shared__ float s_scale[2][SWIGLU_SCALES];      // [up, gate][group][row]
     const int groups = I >> 7, sub = threadIdx.x & 7;
@@ -166,9 +168,9 @@ __global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_save_kernel(const T* __
     const int nr = min(1 << rsh, live - r0), nj = min(gpc, groups - j0);
     if (nr <= 0) return;
     const int total = nr * nj;
-    BlockWalk at(nj);
+    BlockWalk<SAVE_TURN> at(nj);
     // the trip count is the same for all lanes (the shuffles name the warp)
-    for (int i0 = 0; i0 < total; i0 += SWIGLU_TURN, at.step()) {
+    for (int i0 = 0; i0 < total; i0 += SAVE_TURN, at.step()) {
         const bool on = at.r < nr;
         const size_t col = (size_t)(j0 + at.j) * 128 + sub * 16, row = r0 + at.r;
         Cols<T> up, gate;
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_save_kernel(const T* __
     }
     __syncthreads();
     pdl_launch();
-    for (int i = threadIdx.x; i < nj << rsh; i += SWIGLU_THREADS) {
+    for (int i = threadIdx.x; i < nj << rsh; i += SAVE_THREADS) {
         const int j = i >> rsh, r = i - (j << rsh);
         if (r < nr) {
             scale[(size_t)(j0 + j) * rows + r0 + r] = s_scale[0][i];
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_save_kernel(const T* __
 }
 
 template <typename T, bool ACT>
-__global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_grad_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ d_act,
+__global__ void __launch_bounds__(GRAD_X_THREADS) swiglu_grad_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ d_act,
                                                                      const int32_t* __restrict__ used, int rows, int I, int rsh, int gpc,
                                                                      T* __restrict__ d_x, T* __restrict__ act) {
     const int groups = I >> 7, sub = threadIdx.x & 7;
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(SWIGLU_THREADS) swiglu_grad_kernel(const uint8
     const int live = used ? min(__ldg(used), rows) : rows;
     const int nr = min(1 << rsh, live - r0), nj = min(gpc, groups - j0);
     const int total = nr > 0 ? nr * nj : 0;
-    BlockWalk at(max(nj, 1));
-    for (int i = threadIdx.x >> 3; i < total; i += SWIGLU_TURN, at.step()) {
+    BlockWalk<GRAD_X_TURN> at(max(nj, 1));
+    for (int i = threadIdx.x >> 3; i < total; i += GRAD_X_TURN, at.step()) {
         const size_t col = (size_t)(j0 + at.j) * 128 + sub * 16, row = r0 + at.r;
         const uint4 qu = __ldg(reinterpret_cast<const uint4*>(q + row * 2 * I + col)), qg = __ldg(reinterpret_cast<const uint4*>(q + row * 2 * I + I + col));
         const float su = __ldg(scale + (size_t)(j0 + at.j) * rows + row), sg = __ldg(scale + (size_t)(groups + j0 + at.j) * rows + row);

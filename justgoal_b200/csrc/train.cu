@@ -95,21 +95,23 @@ int restore_rows(const OrderParams& o, const void* q, const float* scale, void* 
 }
 
 // Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; fewer rows where that leaves less than two CTAs per SM.
-// save: the fewest rows, four at least (half a sector of scales), that keep the CTA's threads busy in four fifths of its turns.  Two / four / eight rows
-// of 2048 columns, us: 2000 rows 7.4 / 7.2 / 9.2, 8000: 24.4 / 23.6 / 24.3, 34645: 93.8 / 88.6 / 89.8; eight / 16 / 32 of 640 columns (five groups: 62, 83
-// and 100 %) 40000 rows 42.0 / 38.0 / 38.8.
+// save: the fewest rows, two at least (scales leave as runs of rows), that keep the CTA's threads busy in four fifths of its turns.  One / two / four rows
+// of 2048 columns, us: 2000 rows 6.8 / 6.7 / 8.7, 8000: 23.3 / 23.1 / 23.2, 34645: 90.0 / 87.6 / 88.5; four / eight / 16 of 640 columns (five groups: 62, 83
+// and 100 %) 40000 rows 38.8 / 35.7 / 37.4; four / eight / 16 of 256 columns 20000 rows 11.8 / 9.2 / 9.8.
+// (256 threads per CTA: level for 2048 columns, 93.5 against 91.9 under the clocks of a long run, 40000 x 640 37.8, 20000 x 256 9.6.)
 // backward: nothing is kept between turns, so about one turn: two / four / eight rows of 2048 columns 8000 rows 26.7 / 27.4 / 28.2, 34645: 106.0 / 108.3 /
-// 110.6; four / eight / 16 of 640 columns 40.0 / 41.2 / 42.2; eight / 16 of 256 columns 20000 rows 10.1 / 10.2.
+// 110.6; four / eight / 16 of 640 columns 40.0 / 41.2 / 42.2; eight / 16 of 256 columns 20000 rows 10.1 / 10.2.  (128 threads per CTA with half
+// the rows: level, 109.6 against 108.1 in a long run.)
 void swiglu_block(bool save, int rows, int I, int& rsh, int& gpc, dim3& grid) {
     const int groups = I >> 7, parts = (groups + 63) / 64;
     gpc = (groups + parts - 1) / parts;
     if (save) {
-        for (rsh = 2; rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES; ++rsh) {
-            const int items = gpc << rsh, turns = (items + SWIGLU_TURN - 1) / SWIGLU_TURN;
-            if (items * 5 >= turns * SWIGLU_TURN * 4) break;
+        for (rsh = 1; rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES; ++rsh) {
+            const int items = gpc << rsh, turns = (items + SAVE_TURN - 1) / SAVE_TURN;
+            if (items * 5 >= turns * SAVE_TURN * 4) break;
         }
     } else {
-        for (rsh = 0; rsh < 5 && (gpc << rsh) * 8 < SWIGLU_TURN * 5; ++rsh) {}
+        for (rsh = 0; rsh < 5 && (gpc << rsh) * 8 < GRAD_X_TURN * 5; ++rsh) {}
     }
     while (rsh > 0 && (long long)((rows + (1 << rsh) - 1) >> rsh) * parts < 2ll * sm_count()) --rsh;
     grid = dim3((rows + (1 << rsh) - 1) >> rsh, (groups + gpc - 1) / gpc);
@@ -120,7 +122,7 @@ int swiglu_save(const void* x, const int32_t* used, int rows, int I, void* act, 
     int rsh, gpc;
     dim3 grid;
     swiglu_block(true, rows, I, rsh, gpc, grid);
-    return launch(swiglu_save_kernel<T>, grid, SWIGLU_THREADS, stream, static_cast<const T*>(x), used, rows, I, rsh, gpc, static_cast<T*>(act),
+    return launch(swiglu_save_kernel<T>, grid, SAVE_THREADS, stream, static_cast<const T*>(x), used, rows, I, rsh, gpc, static_cast<T*>(act),
                   static_cast<uint8_t*>(q), scale);
 }
 
@@ -129,7 +131,7 @@ int swiglu_grad(const void* q, const float* scale, const void* d_act, const int3
     int rsh, gpc;
     dim3 grid;
     swiglu_block(false, rows, I, rsh, gpc, grid);
-    return launch(act ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>, grid, SWIGLU_THREADS, stream, static_cast<const uint8_t*>(q), scale,
+    return launch(act ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>, grid, GRAD_X_THREADS, stream, static_cast<const uint8_t*>(q), scale,
                   static_cast<const T*>(d_act), used, rows, I, rsh, gpc, static_cast<T*>(d_x), static_cast<T*>(act));
 }
 
