@@ -302,30 +302,34 @@ __device__ __forceinline__ void token_rows(const OrderParams& o, int t, int* r) 
         if (r[k] >= o.num_rows) r[k] = -1;
 }
 
-// Zeros into the padding rows of the segments.  Every warp owns a block of up to 32 consecutive rows (several where there are more rows than
-// that).  Which rows of the first block are padding is looked up early (begin) and acted on behind the kernel's own work, so that
-// the look-up's latency hides.
+// Zeros into the padding rows of the segments: rows in use whose pair is none of the T K (-1, or an id of another call's tables).  Every warp owns a
+// block of up to 32 consecutive rows (several where there are more rows than that).  Which rows of the first block are padding is looked up
+// early (begin) and acted on behind the kernel's own work, so that the look-up's latency hides.
 struct Padding {
-    int used, pair;
+    int used;
+    bool empty;                                        // this lane's row of the block
     static __device__ __forceinline__ int warp() { return (int)((blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x) >> 5); }
     static __device__ __forceinline__ int warps() { return (int)((gridDim.x * (unsigned long long)blockDim.x) >> 5); }
     static __device__ __forceinline__ int per(const OrderParams& o) { return min(32, (o.num_rows - 1) / warps() + 1); }
+    __device__ __forceinline__ void look(const OrderParams& o, long long r0, int n) {
+        const int lane = threadIdx.x & 31;
+        empty = lane < n && r0 + lane < used && (unsigned)__ldg(o.row_pair + r0 + lane) >= (unsigned)(o.T * o.top_k);
+    }
     __device__ __forceinline__ void begin(const OrderParams& o) {
         used = min(__ldg(o.expert_row0 + o.num_local), o.num_rows);
-        const int lane = threadIdx.x & 31, n = per(o);
-        const long long r = (long long)warp() * n + lane;
-        pair = lane < n && r < used ? __ldg(o.row_pair + r) : 0;
+        const int n = per(o);
+        look(o, (long long)warp() * n, n);
     }
     __device__ __forceinline__ void fill(const OrderParams& o, char* rows, int units) {
         const int lane = threadIdx.x & 31, n = per(o);
         for (long long r0 = (long long)warp() * n;;) {
-            for (unsigned empty = __ballot_sync(0xFFFFFFFFu, pair < 0); empty; empty &= empty - 1) {
-                char* dst = rows + (size_t)(r0 + __ffs(empty) - 1) * units * 32;
+            for (unsigned left = __ballot_sync(0xFFFFFFFFu, empty); left; left &= left - 1) {
+                char* dst = rows + (size_t)(r0 + __ffs(left) - 1) * units * 32;
                 for (int u = lane; u < units; u += 32) st_global_v8(dst + (size_t)u * 32, 0, 0, 0, 0, 0, 0, 0, 0);
             }
             r0 += (long long)warps() * n;
             if (r0 >= used) break;
-            pair = lane < n && r0 + lane < used ? __ldg(o.row_pair + r0 + lane) : 0;
+            look(o, r0, n);
         }
     }
 };
@@ -523,7 +527,7 @@ __device__ __forceinline__ void combine_grad_by_rows(const OrderParams& o, const
     int next = r_first < used ? __ldg(o.row_pair + r_first) : -1;          // the next row's pair, looked up one turn ahead
     for (long long r0 = (long long)blockIdx.x * groups; r0 < used; r0 += step, buf ^= 1) {
         const long long r = r0 + (threadIdx.x >> gsh);
-        const int pair = next < pairs ? next : -1;
+        const int pair = next < pairs ? next : -1;                            // (negative: none)
         next = r + step < used ? __ldg(o.row_pair + r + step) : -1;
         float dot = 0.f;
         if (r < used) {

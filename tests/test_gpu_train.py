@@ -931,3 +931,33 @@ def test_swiglu_and_gradients_past_32_bits():
     assert not bool(grad[R - 2].any()) and not bool(grad[2].any()) and float(grad_w[0, 1]) == 0.0
     dot = (g[0].double() * x[R - 1].double()).sum()
     assert abs(float(grad_w[0, 0]) - float(dot)) <= (2 * inner / 32 + 13) * U * float((g[0].double() * x[R - 1].double()).abs().sum())
+
+
+# ------------------------------------------------------------------ orders cut to fewer tokens
+
+@pytest.mark.parametrize("T,all_T", [(20, 40), (400, 500)])          # (the combine's gradient by rows and by tokens)
+def test_rows_of_pairs_that_the_call_does_not_have_are_padding(T, all_T):
+    """A row in use whose pair is none of the call's T * top_k counts like -1: zeros from every operator that writes rows."""
+    from justgoal_b200 import TokenOrder, combine_backward, permute, quantize_1x128, restore_1x128
+    K, H = 8, 256
+    whole, tables = _order(all_T, K, 32, seed=T)
+    order = TokenOrder(whole.expert_row0, whole.row_pair, whole.pair_row[:T])
+    row0, row_pair, _ = tables
+    used, R = int(row0[-1]), row_pair.numel()
+    assert (used > 3 * T and T > 256) == (T == 400)
+    here = (row_pair >= 0) & (row_pair < T * K)
+    pair = row_pair[here].long()
+    x, rows, w = _rows(T, H, torch.bfloat16, 1), _rows(R, H, torch.bfloat16, 2), torch.rand(T, K, generator=_gen(3))
+    q, scale = quantize_1x128(x)
+    flat = (q.cpu().float().view(T, H // 128, 128) * scale.cpu().t()[:, :, None]).view(T, H).to(torch.bfloat16)
+    out = torch.empty(R, H, dtype=torch.bfloat16, device="cuda")
+    for name, call, value in (("permute", lambda: permute(x, order, out=out), x.cpu()[pair // K]),
+                              ("restore", lambda: restore_1x128(q, scale, order, out=out), flat[pair // K]),
+                              ("combine", lambda: combine_backward(x, rows, w.cuda(), order, out=out),
+                               (x.cpu()[pair // K].float() * w.flatten()[pair][:, None]).to(torch.bfloat16))):
+        out.fill_(float("nan"))
+        call()
+        want = torch.full((R, H), float("nan"), dtype=torch.bfloat16)
+        want[:used] = 0
+        want[here] = value
+        assert torch.equal(out.cpu().view(torch.int16), want.view(torch.int16)), name
