@@ -18,7 +18,8 @@ Every call runs on the current stream of its tensors' device, whichever device i
 counts in `sort_tokens`), keeps nothing, and can be captured into a CUDA graph.  Row tensors are bf16, fp16 or fp32; tensors that are not contiguous, or do
 not start at a 32-byte boundary, are copied first (`out` tensors are refused).  Row tensors have room for `order.row_pair.numel()` rows:
 `permute`, `restore_1x128`, `combine_backward` and the SwiGLU pair write the rows in use, padding of the segments included (as zeros), and leave
-those behind `expert_row0[-1]` as they were (unset where the call makes the tensor).  The gradients are plain functions: autograd does not record these calls.
+those behind `expert_row0[-1]` as they were (unset where the call makes the tensor).  The gradients are plain functions: autograd does not record these calls.  A call that
+writes an `out` tensor counts as a change of it in place: a backward pass that had saved it raises, as after any change in place.
 """
 from __future__ import annotations
 
@@ -36,6 +37,7 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ALIGN = 32
 _I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_written = torch.autograd.graph.increment_version      # the caller's tensors changed: autograd refuses a backward pass that had saved them
 
 
 @functools.lru_cache(maxsize=1024)
@@ -172,12 +174,15 @@ def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = No
     order, row0, row_pair, pair_row, T, K, El, R = _order(order, device)
     if n != T:
         _off(x, "x", x.dtype, (T, H))
-    if out is None:
+    made = out is None
+    if made:
         out = x.new_empty((R, H))
         at = out.data_ptr()
     else:
         at = _given(out, "out", device, x.dtype, (R, H), _ALIGN, x)
     _call(_lib.lib.b200moe_permute, device, x_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
+    if not made:
+        _written(out)
     return out
 
 
@@ -187,12 +192,15 @@ def _combine(rows, w, order, out):
     if n != R:
         _off(rows, "rows", rows.dtype, (R, H))
     w, w_at = (None, None) if w is None else _in(w, "topk_w", device, _F32, (T, K))
-    if out is None:
+    made = out is None
+    if made:
         out = rows.new_empty((T, H))
         at = out.data_ptr()
     else:
         at = _given(out, "out", device, rows.dtype, (T, H), _ALIGN, rows)
     _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row, T, K, H, R, at)
+    if not made:
+        _written(out)
     return out
 
 
@@ -216,13 +224,16 @@ def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.T
         _off(rows, "rows", rows.dtype, (R, H))
     grad_out, grad_at = _in(grad_out, "grad_out", device, rows.dtype, (T, H), _ALIGN)
     topk_w, w_at = _in(topk_w, "topk_w", device, _F32, (T, K))
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(rows)
         at = out.data_ptr()
     else:
         at = _given(out, "out", device, rows.dtype, (R, H), _ALIGN, rows, grad_out)
     grad_w = torch.empty_like(topk_w)
     _call(_lib.lib.b200moe_combine_backward, device, grad_at, rows_at, kind, w_at, row0, row_pair, pair_row, T, K, El, H, R, at, grad_w.data_ptr())
+    if not made:
+        _written(out)
     return out, grad_w
 
 
@@ -250,12 +261,15 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
         order, row0, row_pair, pair_row, tokens, K, El, R = _order(order, device)
         if tokens != T:
             raise ValueError(f"q has {T} tokens, the order {tokens}")
-    if out is None:
+    made = out is None
+    if made:
         out = q.new_empty((R, H), dtype=dtype)
         at = out.data_ptr()
     else:
         at = _given(out, "out", device, dtype, (R, H), _ALIGN, q, scale)
     _call(_lib.lib.b200moe_restore_1x128, device, q_at, scale_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
+    if not made:
+        _written(out)
     return out
 
 
@@ -287,6 +301,8 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
         q_at = _given(q, "q", device, _E4M3, (R, I2), 16, x, act)
         scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), 4, x, act, q)
     _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act_at, q_at, scale_at)
+    if out is not None:
+        _written((act, q, scale))
     return act, q, scale
 
 
@@ -308,6 +324,8 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
         grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), _ALIGN, q, scale, d)
         act_at = _given(act, "act", device, d.dtype, (R, I), _ALIGN, q, scale, d, grad_x) if with_act else None
     _call(_lib.lib.b200moe_swiglu_backward, device, q_at, scale_at, d_at, kind, used, R, I, grad_at, act_at)
+    if out is not None:
+        _written((grad_x, act) if with_act else grad_x)
     return grad_x, act
 
 
@@ -328,10 +346,13 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
     bias, bias_at = (None, None) if routing_bias is None else _in(routing_bias, "routing_bias", device, torch.bfloat16, (E,))
     topk_idx, idx_at = _in(topk_idx, "topk_idx", device, _I32, (T, K))
     grad_w, grad_at = _in(grad_w, "grad_w", device, _F32, (T, K))
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(logits)
         at = out.data_ptr()
     else:
         at = _given(out, "out", device, _F32, (T, E), 16, logits, grad_w)
     _call(_lib.lib.b200moe_route_backward, device, logits_at, bias_at, idx_at, grad_at, T, E, K, float(routed_scaling_factor), routing_mode, at)
+    if not made:
+        _written(out)
     return out

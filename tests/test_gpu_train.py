@@ -961,3 +961,61 @@ def test_rows_of_pairs_that_the_call_does_not_have_are_padding(T, all_T):
         want[:used] = 0
         want[here] = value
         assert torch.equal(out.cpu().view(torch.int16), want.view(torch.int16)), name
+
+
+# ------------------------------------------------------------------ outputs that autograd knows
+
+def _calls_with_outputs():
+    """(name, the outputs, a call that writes them, the call's inputs) for every operator that takes `out`."""
+    import justgoal_b200 as jg
+    T, K, H, E = 20, 4, 256, 64
+    order, tables = _order(T, K, 32, seed=3)
+    R, dtype = tables[1].numel(), torch.bfloat16
+    x, rows, w, d = _rows(T, H, dtype, 1), _rows(R, H, dtype, 2), torch.rand(T, K, device="cuda"), _rows(R, H // 2, dtype, 3)
+    q8, s8 = jg.quantize_1x128(x)
+    _, q, scale = jg.swiglu_save(rows)
+    logits, idx = torch.zeros(T, E, device="cuda"), torch.zeros(T, K, dtype=torch.int32, device="cuda")
+    new = lambda *shape, dtype=dtype: torch.zeros(*shape, dtype=dtype, device="cuda")   # noqa: E731
+    to_rows, to_tokens, to_act, to_q, to_scale = new(R, H), new(T, H), new(R, H // 2), torch.zeros_like(q), torch.zeros_like(scale)
+    to_logits = new(T, E, dtype=torch.float32)
+    return [("permute", (to_rows,), lambda: jg.permute(x, order, out=to_rows), (x, *order)),
+            ("permute_backward", (to_tokens,), lambda: jg.permute_backward(rows, order, out=to_tokens), (rows, *order)),
+            ("combine", (to_tokens,), lambda: jg.combine(rows, w, order, out=to_tokens), (rows, w, *order)),
+            ("combine_backward", (to_rows,), lambda: jg.combine_backward(x, rows, w, order, out=to_rows), (x, rows, w, *order)),
+            ("restore_1x128", (to_rows,), lambda: jg.restore_1x128(q8, s8, order, out=to_rows), (q8, s8, *order)),
+            ("swiglu_save", (to_act, to_q, to_scale), lambda: jg.swiglu_save(rows, order.expert_row0, out=(to_act, to_q, to_scale)),
+             (rows, order.expert_row0)),
+            ("swiglu_backward", (to_rows, to_act), lambda: jg.swiglu_backward(q, scale, d, order.expert_row0, out=(to_rows, to_act)),
+             (q, scale, d, order.expert_row0)),
+            ("swiglu_backward without act", (to_rows,), lambda: jg.swiglu_backward(q, scale, d, with_act=False, out=(to_rows, None)), (q, scale, d)),
+            ("route_backward", (to_logits,), lambda: jg.route_backward(logits, None, idx, w, 1.0, out=to_logits), (logits, idx, w))]
+
+
+def test_written_outputs_count_as_changed():
+    for name, outs, call, ins in _calls_with_outputs():
+        before, kept = [t._version for t in outs], [t._version for t in ins]
+        call()
+        assert all(t._version > v for t, v in zip(outs, before)), name
+        assert [t._version for t in ins] == kept, name
+
+
+def test_a_saved_tensor_that_is_written_again_stops_the_backward_pass():
+    """A buffer that a forward pass saved and a later call wrote: the backward pass raises instead of using the new values."""
+    import justgoal_b200 as jg
+    order, tables = _order(20, 4, 32, seed=4)
+    rows, x = _rows(tables[1].numel(), 256, torch.float32, 1), _rows(20, 256, torch.float32, 2)
+    weight = torch.ones(256, device="cuda", requires_grad=True)
+    loss = (rows * weight).sum()              # saves `rows` for the weight's gradient
+    jg.permute(x, order, out=rows)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_a_refused_call_changes_nothing():
+    import justgoal_b200 as jg
+    rows = _rows(8, 256, torch.bfloat16, 1)
+    act, q = torch.zeros(8, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(8, 256, device="cuda").to(torch.float8_e4m3fn)
+    before = act._version, q._version
+    with pytest.raises(ValueError):
+        jg.swiglu_save(rows, out=(act, q, torch.zeros(3, 8, device="cuda")))
+    assert (act._version, q._version) == before
