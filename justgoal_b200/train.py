@@ -111,14 +111,14 @@ def _rows(t, name, columns=128):
 
 def _given(t, name, device, dtype, shape, align, *others):
     """The address of the caller's output, which has to be of the form that is written in place and share no memory with the call's
-    rows and other outputs."""
+    inputs and other outputs (tensors, or addresses with their numbers of bytes)."""
     at = t.data_ptr()
     if t.dtype is not dtype or t.shape != shape or t.get_device() != device or at % align or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on cuda:{device} that starts at a multiple of {align} bytes")
     end = at + t.nbytes
     for other in others:
-        start = other.data_ptr()
-        if start < end and at < start + other.nbytes and at < end:
+        start, n = other if type(other) is tuple else (other.data_ptr(), other.nbytes)
+        if start < end and at < start + n and at < end:
             raise ValueError(f"{name} must not share memory with an input or another output")
     return at
 
@@ -179,7 +179,7 @@ def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = No
         out = x.new_empty((R, H))
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, x.dtype, (R, H), _ALIGN, x)
+        at = _given(out, "out", device, x.dtype, (R, H), _ALIGN, x, (row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
     _call(_lib.lib.b200moe_permute, device, x_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
     if not made:
         _written(out)
@@ -197,7 +197,7 @@ def _combine(rows, w, order, out):
         out = rows.new_empty((T, H))
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, rows.dtype, (T, H), _ALIGN, rows)
+        at = _given(out, "out", device, rows.dtype, (T, H), _ALIGN, rows, (pair_row, 4 * T * K), (w_at or 0, 0 if w is None else 4 * T * K))
     _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row, T, K, H, R, at)
     if not made:
         _written(out)
@@ -229,7 +229,7 @@ def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.T
         out = torch.empty_like(rows)
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, rows.dtype, (R, H), _ALIGN, rows, grad_out)
+        at = _given(out, "out", device, rows.dtype, (R, H), _ALIGN, rows, grad_out, topk_w, (row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
     grad_w = torch.empty_like(topk_w)
     _call(_lib.lib.b200moe_combine_backward, device, grad_at, rows_at, kind, w_at, row0, row_pair, pair_row, T, K, El, H, R, at, grad_w.data_ptr())
     if not made:
@@ -266,7 +266,8 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
         out = q.new_empty((R, H), dtype=dtype)
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, dtype, (R, H), _ALIGN, q, scale)
+        tables = () if order is None else ((row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
+        at = _given(out, "out", device, dtype, (R, H), _ALIGN, q, scale, *tables)
     _call(_lib.lib.b200moe_restore_1x128, device, q_at, scale_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
     if not made:
         _written(out)
@@ -297,9 +298,10 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
         act_at, q_at, scale_at = act.data_ptr(), q.data_ptr(), scale.data_ptr()
     else:
         act, q, scale = out
-        act_at = _given(act, "act", device, x.dtype, (R, I2 // 2), _ALIGN, x)
-        q_at = _given(q, "q", device, _E4M3, (R, I2), 16, x, act)
-        scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), 4, x, act, q)
+        ins = (x,) if keep is None else (x, keep)
+        act_at = _given(act, "act", device, x.dtype, (R, I2 // 2), _ALIGN, *ins)
+        q_at = _given(q, "q", device, _E4M3, (R, I2), 16, *ins, act)
+        scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), 4, *ins, act, q)
     _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act_at, q_at, scale_at)
     if out is not None:
         _written((act, q, scale))
@@ -321,8 +323,9 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
         grad_x, act = out
         if (act is not None) != with_act:
             raise ValueError("out has a tensor for act if and only if with_act asks for it")
-        grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), _ALIGN, q, scale, d)
-        act_at = _given(act, "act", device, d.dtype, (R, I), _ALIGN, q, scale, d, grad_x) if with_act else None
+        ins = (q, scale, d) if keep is None else (q, scale, d, keep)
+        grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), _ALIGN, *ins)
+        act_at = _given(act, "act", device, d.dtype, (R, I), _ALIGN, *ins, grad_x) if with_act else None
     _call(_lib.lib.b200moe_swiglu_backward, device, q_at, scale_at, d_at, kind, used, R, I, grad_at, act_at)
     if out is not None:
         _written((grad_x, act) if with_act else grad_x)
@@ -351,7 +354,7 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
         out = torch.empty_like(logits)
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, _F32, (T, E), 16, logits, grad_w)
+        at = _given(out, "out", device, _F32, (T, E), 16, logits, grad_w, topk_idx, *(() if bias is None else (bias,)))
     _call(_lib.lib.b200moe_route_backward, device, logits_at, bias_at, idx_at, grad_at, T, E, K, float(routed_scaling_factor), routing_mode, at)
     if not made:
         _written(out)

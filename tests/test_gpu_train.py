@@ -1019,3 +1019,52 @@ def test_a_refused_call_changes_nothing():
     with pytest.raises(ValueError):
         jg.swiglu_save(rows, out=(act, q, torch.zeros(3, 8, device="cuda")))
     assert (act._version, q._version) == before
+
+
+def _forms_with_outputs():
+    """name -> (inputs, outputs, call of both lists) for every operator that takes `out`; a call that lets an output lie over an input is refused
+    before anything runs."""
+    import justgoal_b200 as jg
+    T, K, H, E = 20, 4, 256, 64
+    order, tables = _order(T, K, 32, seed=3)
+    R, bf16, f32 = tables[1].numel(), torch.bfloat16, torch.float32
+    new = lambda *shape, dtype=bf16: torch.zeros(*shape, dtype=dtype, device="cuda")   # noqa: E731
+    eight = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)   # noqa: E731
+    w, logits, bias, idx = new(T, K, dtype=f32), new(T, E, dtype=f32), new(E), new(T, K, dtype=torch.int32)
+    q8, s8, q, scale = eight(T, H), new(H // 128, T, dtype=f32), eight(R, H), new(H // 128, R, dtype=f32)
+    t = jg.TokenOrder
+    return {
+        "permute": ([new(T, H), *order], [new(R, H)], lambda i, o: jg.permute(i[0], t(*i[1:]), out=o[0])),
+        "permute_backward": ([new(R, H), order[2]], [new(T, H)], lambda i, o: jg.permute_backward(i[0], t(*order[:2], i[1]), out=o[0])),
+        "combine": ([new(R, H), w, order[2]], [new(T, H)], lambda i, o: jg.combine(i[0], i[1], t(*order[:2], i[2]), out=o[0])),
+        "combine_backward": ([new(T, H), new(R, H), w, *order], [new(R, H)], lambda i, o: jg.combine_backward(*i[:3], t(*i[3:]), out=o[0])),
+        "restore_1x128": ([q8, s8, *order], [new(R, H)], lambda i, o: jg.restore_1x128(*i[:2], t(*i[2:]), out=o[0])),
+        "restore_1x128 plain": ([q8, s8], [new(T, H)], lambda i, o: jg.restore_1x128(*i, out=o[0])),
+        "swiglu_save": ([new(R, H), order[0]], [new(R, H // 2), eight(R, H), new(H // 128, R, dtype=f32)], lambda i, o: jg.swiglu_save(*i, out=tuple(o))),
+        "swiglu_backward": ([q, scale, new(R, H // 2), order[0]], [new(R, H), new(R, H // 2)], lambda i, o: jg.swiglu_backward(*i, out=tuple(o))),
+        "route_backward": ([logits, bias, idx, w], [new(T, E, dtype=f32)], lambda i, o: jg.route_backward(*i, 1.0, out=o[0]))}
+
+
+@pytest.mark.parametrize("name", ["permute", "permute_backward", "combine", "combine_backward", "restore_1x128", "restore_1x128 plain", "swiglu_save",
+                                  "swiglu_backward", "route_backward"])
+def test_outputs_over_any_input_are_refused(name):
+    """Tables, weights, ids and biases as well as rows, and the other outputs: at an output's first bytes and at its last."""
+    ins, outs, call = _forms_with_outputs()[name]
+    call(ins, outs)                                                     # (apart from each other they are taken)
+
+    def both(a, b, at):                                                 # the two in one buffer, b at byte `at` of a
+        room = torch.zeros(at + b.nbytes + a.nbytes, dtype=torch.uint8, device="cuda")
+        return room[:a.nbytes].view(a.dtype).view(a.shape), room[at:at + b.nbytes].view(b.dtype).view(b.shape)
+
+    for k, out in enumerate(outs):
+        for at in (0, (out.nbytes - 1) // 32 * 32):
+            for j, t in enumerate(ins):
+                o, i = list(outs), list(ins)
+                o[k], i[j] = both(out, t, at)
+                with pytest.raises(ValueError, match="share memory"):
+                    call(i, o)
+            for j in range(k):
+                o = list(outs)
+                o[k], o[j] = both(out, outs[j], at)
+                with pytest.raises(ValueError, match="share memory"):
+                    call(ins, o)
