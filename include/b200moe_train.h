@@ -33,7 +33,9 @@ extern "C" {
  *   pair_row    int32 [T, top_k]       row of a pair, -1 where it has none
  * max_rows >= T * top_k + (align - 1) * num_local holds every case.  With less, pairs whose row would lie behind it get none (as if
  * their expert were elsewhere), and expert_row0 ends at max_rows.
- * workspace: b200moe_sort_workspace_bytes(T, top_k, num_local) bytes, 16-byte aligned (none for up to 2048 pairs). */
+ * workspace: b200moe_sort_workspace_bytes(T, top_k, num_local) bytes, 16-byte aligned (none for up to 2048 pairs).  That is enough for every call with
+ * no more pairs (T * top_k) and no more local experts.  It depends on the number of SMs of the device that is current: ask with the device current
+ * that sorts. */
 int b200moe_sort_workspace_bytes(int num_tokens, int top_k, int num_local, size_t* bytes);
 int b200moe_sort_tokens(const int32_t* topk_idx, int num_tokens, int top_k, int num_local, int local_offset, int align, int max_rows,
                         int32_t* expert_row0, int32_t* row_pair, int32_t* pair_row, void* workspace, size_t workspace_bytes,

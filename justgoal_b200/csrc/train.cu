@@ -46,6 +46,12 @@ size_t sort_bytes(int n, int num_local) {
     const int ctas = sort_ctas(n);
     return ctas > 1 ? (size_t)ctas * sort_pitch(num_local) * sizeof(int) : 0;
 }
+// What a caller is told: enough for this size and every smaller one.  (Slices grow by whole SORT_THREADS, so that the CTAs of a call, and with them
+// sort_bytes, fall where a slice takes one pair per thread more: on 148 SMs 296 CTAs for 303104 pairs, 149 for 303112.)
+size_t sort_bytes_upto(int n, int num_local) {
+    const size_t ctas = n <= SORT_ALONE ? 0 : min((n + SORT_THREADS - 1) / SORT_THREADS, 2 * sm_count());
+    return ctas * sort_pitch(num_local) * sizeof(int);
+}
 
 constexpr int MAX_COLUMNS = 1 << 20, MAX_ROWS = 1 << 30;      // (index arithmetic stays in range; far above what a GPU's memory holds)
 
@@ -143,7 +149,7 @@ extern "C" {
 
 int b200moe_sort_workspace_bytes(int T, int top_k, int num_local, size_t* bytes) {
     if (!bytes || bad_picks(T, top_k) || num_local < 1 || num_local > ORDER_MAX_LOCAL) return B200MOE_E_BADARG;
-    *bytes = sort_bytes(T * top_k, num_local);
+    *bytes = sort_bytes_upto(T * top_k, num_local);
     return 0;
 }
 

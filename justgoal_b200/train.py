@@ -42,7 +42,7 @@ _written = torch.autograd.graph.increment_version      # the caller's tensors ch
 
 @functools.lru_cache(maxsize=1024)
 def _sort_bytes(T, K, El, device):
-    """Workspace of b200moe_sort_tokens over these sizes on that device."""
+    """Workspace of b200moe_sort_tokens over these sizes (and smaller ones) on that device."""
     n = C.c_size_t()
     with torch.cuda.device(device):
         _lib.check(_lib.lib.b200moe_sort_workspace_bytes(T, K, El, C.byref(n)), "b200moe_sort_workspace_bytes")

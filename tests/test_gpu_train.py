@@ -1068,3 +1068,26 @@ def test_outputs_over_any_input_are_refused(name):
                 o[k], o[j] = both(out, outs[j], at)
                 with pytest.raises(ValueError, match="share memory"):
                     call(ins, o)
+
+
+def test_sort_in_the_workspace_of_a_larger_batch():
+    """One workspace, sized for the largest call, through the C entry point: sizes on both sides of where slices get longer."""
+    import ctypes as C
+    from justgoal_b200 import _lib
+    K, El, most = 8, 64, 37889
+    n = C.c_size_t()
+    assert _lib.lib.b200moe_sort_workspace_bytes(most, K, El, C.byref(n)) == 0
+    room = torch.full((n.value + 64,), 171, dtype=torch.uint8, device="cuda")
+    at = room.data_ptr()
+    assert at % 16 == 0
+    for T in (most, 37888, 300, 20000):
+        idx = _picks(T, K, El, seed=T)
+        R = T * K + 15 * El
+        row0, row_pair, pair_row = (torch.empty(s, dtype=torch.int32, device="cuda") for s in ((El + 1,), (R,), (T, K)))
+        ids = idx.cuda()
+        rc = _lib.lib.b200moe_sort_tokens(ids.data_ptr(), T, K, El, 0, 16, R, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), at, n.value,
+                                          torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, T
+        for g, w in zip((row0, row_pair, pair_row), oracle_order(idx, El)):
+            assert torch.equal(g.cpu(), w)
+        assert bool((room[n.value:] == 171).all())

@@ -120,3 +120,20 @@ def test_python_entry_points_refuse_host_tensors_and_wrong_types():
                  lambda: jg.permute(x[0], order), lambda: jg.combine(rows.int(), w, order), lambda: jg.swiglu_save(rows.to(torch.int8))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_sort_workspace_of_a_size_is_enough_for_smaller_ones():
+    """Never falls with the pairs or the local experts: the CTAs of a call do, where slices get longer (303104, 606208, ... pairs on 148 SMs)."""
+    def size(T, K=8, El=256):
+        n = C.c_size_t()
+        assert lib.b200moe_sort_workspace_bytes(T, K, El, C.byref(n)) == 0
+        return n.value
+
+    steps = [257, 258, 384, 385, 1000, 14107, 37887, 37888, 37889, 40000, 75775, 75776, 75777, 113664, 113665, 1 << 20, 1 << 26, 1 << 27]
+    sizes = [size(T) for T in steps]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    for T in (256, 5000, 37889):
+        by_experts = [size(T, El=El) for El in (1, 4, 5, 32, 255, 256, 512)]
+        assert by_experts == sorted(by_experts)
+    pairs = [size(T, K=1) for T in range(2000, 320000, 333)]
+    assert pairs == sorted(pairs)
