@@ -1091,3 +1091,31 @@ def test_sort_in_the_workspace_of_a_larger_batch():
         for g, w in zip((row0, row_pair, pair_row), oracle_order(idx, El)):
             assert torch.equal(g.cpu(), w)
         assert bool((room[n.value:] == 171).all())
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_swiglu_takes_padding_like_any_row(kind):
+    """Rows in use are computed whether or not a pair stands in them: zeros give zeros, a NaN stays in its own row, all others as without it."""
+    from justgoal_b200 import swiglu_backward, swiglu_save
+    dtype = TYPES[kind]
+    order, (row0, row_pair, _) = _order(10, 4, 32, seed=6)
+    used, R = int(row0[-1]), row_pair.numel()
+    padding = (row_pair < 0) & (torch.arange(R) < used)
+    first, last = padding.nonzero().flatten()[[0, -1]].tolist()
+    x, d = _rows(R, 256, dtype, 1), _rows(R, 128, dtype, 2)
+    x[padding.cuda()] = 0
+    d[padding.cuda()] = 0
+    clean = swiglu_save(x, order.expert_row0)
+    grads = swiglu_backward(clean[1], clean[2], d, order.expert_row0)
+    on = padding.cuda()
+    assert not bool(clean[0][on].any()) and not bool(clean[1][on].float().any()) and bool((clean[2][:, on] == 1).all())
+    assert not bool(grads[0][on].any()) and not bool(grads[1][on].any())
+    x[first] = float("nan")
+    x[last, 200] = float("inf")
+    dirty = swiglu_save(x, order.expert_row0)
+    grads2 = swiglu_backward(dirty[1], dirty[2], d, order.expert_row0)
+    assert bool(dirty[0][first].isnan().all()) and bool(grads2[0][first].isnan().all()) and bool(grads2[1][last].isnan().all())
+    rest = torch.arange(used, device="cuda")
+    rest = rest[(rest != first) & (rest != last)]
+    for a, b in zip((dirty[0], dirty[1].view(torch.uint8), dirty[2].t(), *grads2), (clean[0], clean[1].view(torch.uint8), clean[2].t(), *grads)):
+        assert torch.equal(a[rest], b[rest])
