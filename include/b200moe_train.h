@@ -72,7 +72,8 @@ int b200moe_combine_backward(const void* grad_out, const void* rows, int type, c
  * codes end at 240 under the scale 2^120: a finite value is restored as a finite one).
  * used_rows: device pointer to the number of rows in use (expert_row0 + num_local), NULL = all; the others are left as they were.  Padding of the segments
  * is in use: it is taken like any row here and in the gradient, zeros give zeros, and what is not finite there stays so - the GEMMs around have to
- * leave zeros in it.  (16-bit rows: the sigmoid of a gate below -87 counts as zero.) */
+ * leave zeros in it.  The sigmoid of a gate below -87 leaves fp32's
+ * normal range and counts as zero, here and in the gradient (fp32 rows: it loses bits down to -88.7 and is zero below). */
 int b200moe_swiglu_save(const void* gemm1_rows, int type, const int32_t* used_rows, int num_rows, int intermediate, void* act,
                         void* q_e4m3, float* scale, void* cuda_stream);
 

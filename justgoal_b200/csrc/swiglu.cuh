@@ -27,8 +27,10 @@ constexpr int SAVE_THREADS = 128, SAVE_TURN = SAVE_THREADS / SWIGLU_LANES;      
 constexpr int GRAD_X_THREADS = 256, GRAD_X_TURN = GRAD_X_THREADS / SWIGLU_LANES;
 constexpr int SWIGLU_SCALES = 512;                           // most pairs of groups of a CTA
 
-// Two sigmoids, 1 / (1 + 2^(-g log2 e)).  16-bit rows take the fast exponential and reciprocal, flushed: off by a few units of 2^-23, and zero for
-// gates below -87, where the sigmoid leaves fp32's normal range.  fp32 rows take the accurate ones.
+// Two sigmoids, 1 / (1 + 2^(-g log2 e)).  16-bit rows take the fast exponential and reciprocal, flushed.  The product g log2 e is rounded, which moves the
+// exponent by a share of |g|: the sigmoid is off by a share of (4.5 + 1.2 |g|) 2^-23 at most, 2^-18 at g = -20 and 2^-16 at -87, far below the output's
+// rounding of 2^-8 or 2^-11.  Where the sigmoid leaves fp32's normal range, for gates below -87, it counts as zero.  fp32 rows take the accurate ones:
+// three units of 2^-23 down to -87, fewer bits from there to -88.7, where exp(-g) passes the range, zero below.
 template <typename T>
 __device__ __forceinline__ float2 sigmoid2(float2 g) {
     if constexpr (sizeof(T) == 4) return make_float2(__fdiv_rn(1.0f, 1.0f + expf(-g.x)), __fdiv_rn(1.0f, 1.0f + expf(-g.y)));

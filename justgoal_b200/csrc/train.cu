@@ -84,7 +84,7 @@ int combine_rows(const OrderParams& o, const void* rows, const float* w, void* o
 template <typename T>
 int combine_grad(const OrderParams& o, const void* d_out, const void* rows, const float* w, void* d_rows, float* d_w, int H, void* stream) {
     const int units = H * (int)sizeof(T) / 16;
-    // by tokens: more than one warp from eight units per thread on, up to 128 threads; by rows: one warp, more for few tokens, whose rows do not fill the chip
+    // by tokens: more than one warp where a thread would have more than four units, up to 128 threads; by rows: one warp, more for few tokens, whose rows do not fill the chip
     int token_sh = 5, row_sh = 5;
     while (token_sh < 7 && units > 4 << token_sh) ++token_sh;
     while (o.T <= 64 && row_sh < 7 && units >= 2 * GRAD_FLIGHT << row_sh) ++row_sh;

@@ -1119,3 +1119,32 @@ def test_swiglu_takes_padding_like_any_row(kind):
     rest = rest[(rest != first) & (rest != last)]
     for a, b in zip((dirty[0], dirty[1].view(torch.uint8), dirty[2].t(), *grads2), (clean[0], clean[1].view(torch.uint8), clean[2].t(), *grads)):
         assert torch.equal(a[rest], b[rest])
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_swiglu_gates_where_the_sigmoid_leaves_the_range(kind):
+    """Gates from -84 to -120.  Down to -87 the usual bounds; below, where the sigmoid is under 2^-125, it counts as zero, or has lost bits of its 24
+    (fp32 rows, down to -88.7): an output is off by no more than its own size, and never on the other side of zero."""
+    from justgoal_b200 import swiglu_backward, swiglu_save
+    dtype = TYPES[kind]
+    gates = torch.linspace(-84.0, -120.0, 145)
+    x = torch.empty(145, 256)
+    x[:, :128] = torch.tensor([1.0, -3.0, 0.01, 400.0])[torch.arange(128) % 4]
+    x[:, 128:] = gates[:, None]
+    x = x.to(dtype)
+
+    def check(got, want, gate, usual):
+        _check(got, want, torch.where(gate < -87, want.abs(), usual))
+        assert bool((got.cpu().double() * want >= 0).all())
+
+    act, q, scale = swiglu_save(x.cuda())
+    up, gate = x[:, :128].double(), x[:, 128:].double()
+    want = up * gate * torch.sigmoid(gate)
+    check(act, want, gate, want.abs() * (_sigmoid_error(gate, dtype) + 3 * U))
+    d = torch.tensor([1.0, -0.5])[torch.arange(128) % 2].repeat(145, 1).to(dtype)
+    grad, again = swiglu_backward(q, scale, d.cuda())
+    up, gate, s, d_up, d_gate, want = _grad64(*_copy64(x), d)
+    e = _sigmoid_error(gate, dtype)
+    check(again, want, gate, want.abs() * (e + 4 * U))
+    check(grad[:, :128], d_up, gate, d_up.abs() * (e + 4 * U))
+    check(grad[:, 128:], d_gate, gate, d_gate.abs() * (e + 5 * U) + (d.double() * up * s).abs() * (gate.abs() * (s * e + 2 * U) + U * (1 + gate.abs())))
