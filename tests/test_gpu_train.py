@@ -1148,3 +1148,83 @@ def test_swiglu_gates_where_the_sigmoid_leaves_the_range(kind):
     check(again, want, gate, want.abs() * (e + 4 * U))
     check(grad[:, :128], d_up, gate, d_up.abs() * (e + 4 * U))
     check(grad[:, 128:], d_gate, gate, d_gate.abs() * (e + 5 * U) + (d.double() * up * s).abs() * (gate.abs() * (s * e + 2 * U) + U * (1 + gate.abs())))
+
+
+# ------------------------------------------------------------------ loops of large calls
+
+@pytest.mark.parametrize("T,K,E,H,kind", [
+    # by tokens, more tokens than the grid takes in one turn (2368 CTAs of four tokens, of two, of one), rows of 128 columns among them
+    (9601, 4, 32, 128, "bf16"), (9601, 5, 64, 128, "fp32"), (9602, 4, 32, 128, "fp16"), (400, 8, 32, 128, "bf16"), (300, 6, 64, 128, "fp32"), (9601, 4, 64, 256, "fp16"),
+    (5001, 6, 64, 1152, "bf16"), (4999, 4, 32, 640, "fp32"), (2501, 5, 96, 2176, "bf16"), (2500, 4, 32, 1152, "fp32"), (4750, 8, 256, 384, "bf16"),
+    # by rows, several turns of groups of 32, 64 and 128 threads
+    (256, 8, 256, 128, "bf16"), (64, 8, 256, 2048, "bf16"), (64, 8, 256, 2048, "fp32"), (16, 8, 512, 7168, "fp16"), (9601, 2, 32, 128, "bf16")])
+def test_combine_backward_many_turns(T, K, E, H, kind):
+    test_combine_backward(T, K, E, H, kind, 1)
+
+
+@pytest.mark.parametrize("op", ["permute", "restore", "combine_backward"])
+def test_padding_behind_a_warps_first_block(op):
+    """More rows than 32 per warp of the grid: zeros in those without a pair, the rest as it was."""
+    from justgoal_b200 import TokenOrder, combine_backward, permute, restore_1x128
+    T, R, H = (300, 300001, 128) if op == "combine_backward" else (1, 300001, 128)
+    row_pair = torch.zeros(R, dtype=torch.int32)
+    row_pair[::3] = -1
+    row_pair[-40:] = -1
+    row_pair[1::7] = 2 * T                                   # a pair of another call
+    used = R - 5
+    pair_row = torch.full((T, 1), -1, dtype=torch.int32)
+    pair_row[0] = 250004
+    row_pair[250004] = 0
+    order = TokenOrder(torch.tensor([0, used], dtype=torch.int32, device="cuda"), row_pair.cuda(), pair_row.cuda())
+    x = _rows(T, H, torch.bfloat16, 1)
+    out = torch.full((R, H), 7.0, dtype=torch.bfloat16, device="cuda")
+    if op == "permute":
+        permute(x, order, out=out)
+    elif op == "restore":
+        restore_1x128(x.to(torch.float8_e4m3fn), torch.ones(1, T, device="cuda"), order, out=out)
+        x = x.to(torch.float8_e4m3fn).to(torch.bfloat16)
+    else:
+        combine_backward(x, torch.zeros(R, H, dtype=torch.bfloat16, device="cuda"), torch.ones(T, 1, device="cuda"), order, out=out)
+    want = torch.full((R, H), 7.0, dtype=torch.bfloat16)
+    want[:used][(row_pair[:used] < 0) | (row_pair[:used] >= T)] = 0
+    want[250004] = x[0].cpu()
+    assert torch.equal(out.cpu(), want)
+
+
+# (rows per CTA and groups per row of the walks: several turns, and rows that end inside a block)
+BLOCKS = [(3001, 640, "bf16"), (2499, 640, "fp32"), (5003, 384, "fp16"), (5003, 384, "fp32"), (1001, 1664, "bf16"), (601, 8320, "bf16"), (9501, 128, "fp32")]
+
+
+@pytest.mark.parametrize("R,inner,kind", BLOCKS)
+@pytest.mark.parametrize("part", [1.0, 0.87])
+def test_swiglu_save_of_several_turns(R, inner, kind, part):
+    """As test_swiglu_save.  Gates below -87, which the larger draws hold: the sigmoid counts as zero there (or, in fp32 rows down to -88.7, loses bits of
+    its 24 below the normal range), so the activation, e^-87 of up gate at most, is off by no more than itself."""
+    from justgoal_b200 import swiglu_save
+    dtype, used = TYPES[kind], int(R * part)
+    x = torch.randn(R, 2 * inner, generator=_gen(R)) * torch.exp(torch.randn(2 * inner, generator=_gen(R + 1)))
+    x[0, :128] = 0.0
+    x[R // 2, 5] = -0.0
+    x[R // 2, inner:inner + 128] *= 1e-4
+    x = x.to(dtype)
+    act = torch.full((R, inner), 7.0, dtype=dtype, device="cuda")
+    q = torch.full((R, 2 * inner), 9, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scale = torch.full((2 * inner // 128, R), 7.0, device="cuda")
+    swiglu_save(x.cuda(), torch.tensor([0, used], dtype=torch.int32, device="cuda"), out=(act, q, scale))
+    codes, scales = _copy64(x)
+    assert torch.equal(q.view(torch.uint8).cpu()[:used], codes[:used]) and torch.equal(scale.cpu()[:, :used], scales[:, :used])
+    up, gate = x[:used, :inner].double(), x[:used, inner:].double()
+    want = up * gate * torch.sigmoid(gate)
+    _check(act[:used], want, want.abs() * torch.where(gate < -87, 1.0, _sigmoid_error(gate, dtype) + 3 * U))
+    assert bool((act[used:] == 7).all()) and bool((q.view(torch.uint8)[used:] == 9).all()) and bool((scale[:, used:] == 7).all())
+
+
+@pytest.mark.parametrize("R,inner,kind", BLOCKS)
+@pytest.mark.parametrize("part", [1.0, 0.87])
+def test_swiglu_backward_of_several_turns(R, inner, kind, part):
+    test_swiglu_backward(R, inner, kind, part)
+
+
+@pytest.mark.parametrize("T,K,E,El,off,align", [(160001, 8, 512, 512, 0, 16), (170003, 8, 256, 200, 40, 32), (310001, 8, 512, 509, 2, 1)])
+def test_sort_slices_of_several_chunks(T, K, E, El, off, align):
+    test_sort_tables(T, K, E, El, off, align)
