@@ -305,10 +305,17 @@ __device__ __forceinline__ void token_rows(const OrderParams& o, int t, int* r) 
 // Zeros into the padding rows of the segments: rows in use whose pair is none of the T K (-1, or an id of another call's tables).  Every warp owns a
 // block of up to 32 consecutive rows (several where there are more rows than that).  Which rows of the first block are padding is looked up
 // early (begin) and acted on behind the kernel's own work, so that the look-up's latency hides.
+// APART: the warps of a CTA own blocks that are a grid apart, so that one SM does not get the padding of a whole segment: permute with CTAs of 128 threads one token
+// 2.9 -> 2.3 us, 512 tokens 19.1 -> 18.2.  (The gradient of the combine stores all of its rows by tokens and is better off with blocks side by side: 2500
+// tokens of 128 columns 4.9 us, 6.0 with blocks apart.)
+template <bool APART>
 struct Padding {
     int used;
     bool empty;                                        // this lane's row of the block
-    static __device__ __forceinline__ int warp() { return (int)((blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x) >> 5); }
+    static __device__ __forceinline__ int warp() {
+        if constexpr (APART) return (int)((threadIdx.x >> 5) * gridDim.x + blockIdx.x);
+        return (int)((blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x) >> 5);
+    }
     static __device__ __forceinline__ int warps() { return (int)((gridDim.x * (unsigned long long)blockDim.x) >> 5); }
     static __device__ __forceinline__ int per(const OrderParams& o) { return min(32, (o.num_rows - 1) / warps() + 1); }
     __device__ __forceinline__ void look(const OrderParams& o, long long r0, int n) {
@@ -334,13 +341,11 @@ struct Padding {
     }
 };
 
-// rows[r] = x[t] for the token's rows: a unit is read once and stored up to top_k times.  Nothing is shared inside a CTA, and small ones start and
-// end evenly: 256 / 128 / 64 threads, 1 token 4.0 / 2.8 / 2.7 us, 64: 11.8 / 10.2 / 8.6 (55 MB of padding's zeros beside 7 MB of rows), 8192 tokens of
-// 128 columns 5.5 / 4.9 / 4.8, long calls of wide rows level.
-constexpr int PERMUTE_THREADS = 64;
+// rows[r] = x[t] for the token's rows: a unit is read once and stored up to top_k times.  The CTA's size is the host's choice (unit_block).
+constexpr int PERMUTE_THREADS = 256;         // most threads of a CTA
 __global__ void __launch_bounds__(PERMUTE_THREADS) permute_rows_kernel(const OrderParams o, const char* __restrict__ x, char* __restrict__ rows, int units) {
     pdl_wait();
-    Padding pad;
+    Padding<true> pad;
     pad.begin(o);
     const unsigned long long total = (unsigned long long)o.T * units, step = (unsigned long long)gridDim.x * blockDim.x;
     for (unsigned long long g = blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x; g < total; g += step) {
@@ -374,7 +379,7 @@ __global__ void __launch_bounds__(PERMUTE_THREADS) restore_rows_kernel(const Ord
     pdl_wait();
     const bool ordered = o.pair_row != nullptr;
     const int units = H >> 4;
-    Padding pad;
+    Padding<true> pad;
     if (ordered) pad.begin(o);
     const unsigned long long total = (unsigned long long)o.T * units, step = (unsigned long long)gridDim.x * blockDim.x;
     for (unsigned long long g = blockIdx.x * (unsigned long long)blockDim.x + threadIdx.x; g < total; g += step) {
@@ -629,7 +634,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 4) combine_grad_kernel(const Ord
         combine_grad_by_rows(o, d_out, rows, w, d_rows, d_w, H, row_sh, used, s_dot);
         pdl_launch();
     } else {
-        Padding pad;
+        Padding<false> pad;
         pad.begin(o);
         combine_grad_by_tokens(o, d_out, rows, w, d_rows, d_w, H, token_sh, s_dot);
         pdl_launch();

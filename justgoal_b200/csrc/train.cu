@@ -68,10 +68,19 @@ int check_order(const OrderParams& o, int H) {
 // CTAs that look through the padding of `rows` rows: a row a warp, as long as the chip holds them at once
 long long padding_ctas(long long rows, int warps, int per_sm) { return min((rows + warps - 1) / warps, (long long)per_sm * sm_count()); }
 
-// Grid of a kernel whose threads take one unit of a token's row each
-int unit_grid(long long T, int units, long long pad_rows) {
-    return (int)min(max(max((T * units + PERMUTE_THREADS - 1) / PERMUTE_THREADS, padding_ctas(pad_rows, PERMUTE_THREADS / 32, 1536 / PERMUTE_THREADS)), 1ll),
-                    1ll << 24);
+// CTAs of a kernel whose threads take one unit of a token's row each.  Starting CTAs is what bounds a call that has little to do for each unit: plain
+// rows read back from 8 bits, rows of which few have a place here.  Nothing is shared inside a CTA, so small ones are even where padding is most of the work.
+// us, CTAs of 64 / 128 / 256 threads: 4096 x 7168 plain 31.5 / 17.8 / 18.0, 512 x 7168 plain 4.8 / 3.0 / 2.6; permute of 8192 tokens of 7168 columns on an eighth of
+// the experts 61.6 / 38.9 / 40.3, of 1024 9.3 / 6.3 / 6.5, with every expert here level; 8192 x 128 on an eighth 4.6 / 3.2 / 3.3, with every expert 5.1 / 5.2 / 5.6.
+// Few tokens of wide rows over 256 experts: 64 tokens 9.0 / 10.0 / 11.1, 128: 11.4 / 12.6 / 13.5; of 2048 columns 64 tokens 3.2 / 3.4 / 4.3, 256: 4.3 / 4.8 / 5.7, 1024 on
+// an eighth 5.0 / 3.2 / 2.9; of 256 columns 256 tokens 4.0 / 2.3 / 2.7.  So 256 threads without padding, 64 for wide rows of few tokens (up to 12 CTAs per
+// SM), 128 otherwise.
+int unit_block(long long T, int units, long long pad_rows) {
+    if (pad_rows == 0) return PERMUTE_THREADS;
+    return units >= 128 && T * units <= 12ll * 64 * sm_count() ? 64 : 128;
+}
+int unit_grid(long long T, int units, long long pad_rows, int block) {
+    return (int)min(max(max((T * units + block - 1) / block, padding_ctas(pad_rows, block / 32, 1536 / block)), 1ll), 1ll << 24);
 }
 
 template <typename T>
@@ -96,8 +105,9 @@ int combine_grad(const OrderParams& o, const void* d_out, const void* rows, cons
 
 template <typename T>
 int restore_rows(const OrderParams& o, const void* q, const float* scale, void* rows, int H, void* stream) {
-    return launch(restore_rows_kernel<T>, unit_grid(o.T, H / 16, o.pair_row ? o.num_rows : 0), PERMUTE_THREADS, stream, o,
-                  static_cast<const uint8_t*>(q), scale, static_cast<T*>(rows), H);
+    const int units = H / 16, pad_rows = o.pair_row ? o.num_rows : 0, block = unit_block(o.T, units, pad_rows);
+    return launch(restore_rows_kernel<T>, unit_grid(o.T, units, pad_rows, block), block, stream, o, static_cast<const uint8_t*>(q), scale,
+                  static_cast<T*>(rows), H);
 }
 
 // Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; fewer rows where that leaves less than two CTAs per SM.
@@ -176,8 +186,8 @@ int b200moe_permute(const void* x, int type, const int32_t* expert_row0, const i
     if (!known_type(type) || check_order(o, hidden)) return B200MOE_E_BADARG;
     if (num_rows == 0) return 0;
     if (!expert_row0 || !row_pair || !rows || (T && (!x || !pair_row)) || misaligned(x, 32) || misaligned(rows, 32)) return B200MOE_E_BADARG;
-    const int units = hidden * type_bytes(type) / 32;
-    return launch(permute_rows_kernel, unit_grid(T, units, num_rows), PERMUTE_THREADS, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
+    const int units = hidden * type_bytes(type) / 32, block = unit_block(T, units, num_rows);
+    return launch(permute_rows_kernel, unit_grid(T, units, num_rows, block), block, stream, o, static_cast<const char*>(x), static_cast<char*>(rows), units);
 }
 
 int b200moe_restore_1x128(const void* q, const float* scale, int type, const int32_t* expert_row0, const int32_t* row_pair, const int32_t* pair_row,

@@ -1228,3 +1228,12 @@ def test_swiglu_backward_of_several_turns(R, inner, kind, part):
 @pytest.mark.parametrize("T,K,E,El,off,align", [(160001, 8, 512, 512, 0, 16), (170003, 8, 256, 200, 40, 32), (310001, 8, 512, 509, 2, 1)])
 def test_sort_slices_of_several_chunks(T, K, E, El, off, align):
     test_sort_tables(T, K, E, El, off, align)
+
+
+@pytest.mark.parametrize("T,K,E,H,kind", [(253, 3, 32, 7168, "bf16"), (254, 3, 32, 7168, "bf16"), (888, 2, 32, 2048, "fp16"), (889, 2, 32, 2048, "fp16"), (444, 8, 64, 2048, "fp32"),
+                                          (445, 8, 64, 2048, "fp32"), (100, 8, 256, 1920, "bf16"), (9000, 1, 32, 128, "fp32")])
+def test_rows_on_both_sides_of_the_ctas_sizes(T, K, E, H, kind):
+    """CTAs of 64 and of 128 threads (and of 256, for rows read back without an order)."""
+    test_permute(T, K, E, H, kind, 1)
+    test_permute(T, K, E, H, kind, 4)
+    test_restore(T, K, E, H, kind)
