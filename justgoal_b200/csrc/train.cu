@@ -110,26 +110,34 @@ int restore_rows(const OrderParams& o, const void* q, const float* scale, void* 
                   static_cast<T*>(rows), H);
 }
 
-// Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; fewer rows where that leaves less than two CTAs per SM.
+// Block of a CTA of the SwiGLU kernels, 2^rsh rows of gpc pairs of groups; less where that leaves few CTAs per SM.
 // save: the fewest rows, two at least (scales leave as runs of rows), that keep the CTA's threads busy in four fifths of its turns.  One / two / four rows
-// of 2048 columns, us: 2000 rows 6.8 / 6.7 / 8.7, 8000: 23.3 / 23.1 / 23.2, 34645: 90.0 / 87.6 / 88.5; four / eight / 16 of 640 columns (five groups: 62, 83
-// and 100 %) 40000 rows 38.8 / 35.7 / 37.4; four / eight / 16 of 256 columns 20000 rows 11.8 / 9.2 / 9.8.
+// of 2048 columns, us: 2000 rows 6.7 / 6.3 / 8.3, 34645: 90.2 / 87.8 / 88.8; four / eight / 16 of 640 columns (five groups: 62, 83 and 100 %) 40000 rows
+// 38.8 / 35.7 / 37.4; four / eight / 16 of 256 columns 20000 rows 11.8 / 9.2 / 9.8.  Under four CTAs per SM a block of several turns is halved, first its
+// rows, then its groups: 2000 rows of 640 columns 3.1 (fp32 4.4) against 3.4 (5.4) for a line at two CTAs, 1000 of 2048 fp32 5.5 against 6.6, 5000 of 384 fp32 6.5 against 8.2.
+// A block of one turn stays whole: halves leave threads idle (500 rows of 128 columns 1.9 against 2.2).
 // (256 threads per CTA: level for 2048 columns, 93.5 against 91.9 under the clocks of a long run, 40000 x 640 37.8, 20000 x 256 9.6.)
 // backward: nothing is kept between turns, so about one turn: two / four / eight rows of 2048 columns 8000 rows 26.7 / 27.4 / 28.2, 34645: 106.0 / 108.3 /
-// 110.6; four / eight / 16 of 640 columns 40.0 / 41.2 / 42.2; eight / 16 of 256 columns 20000 rows 10.1 / 10.2.  (128 threads per CTA with half
-// the rows: level, 109.6 against 108.1 in a long run.)
+// 110.6; four / eight / 16 of 640 columns 40.0 / 41.2 / 42.2; eight / 16 of 256 columns 20000 rows 10.1 / 10.2.  (fp32 rows: two / four of 2048 columns 194 / 190,
+// of 1536 155 / 143.  128 threads per CTA with half the rows: level, 109.6 against 108.1 in a long run.)
 void swiglu_block(bool save, int rows, int I, int& rsh, int& gpc, dim3& grid) {
-    const int groups = I >> 7, parts = (groups + 63) / 64;
+    const int groups = I >> 7;
+    int parts = (groups + 63) / 64;
     gpc = (groups + parts - 1) / parts;
+    auto ctas = [&] { return (long long)((rows + (1 << rsh) - 1) >> rsh) * parts; };
     if (save) {
         for (rsh = 1; rsh < 5 && (gpc << (rsh + 1)) <= SWIGLU_SCALES; ++rsh) {
             const int items = gpc << rsh, turns = (items + SAVE_TURN - 1) / SAVE_TURN;
             if (items * 5 >= turns * SAVE_TURN * 4) break;
         }
+        while ((gpc << rsh) > SAVE_TURN && ctas() < 4ll * sm_count()) {
+            if (rsh > 0) --rsh;
+            else { ++parts; gpc = (groups + parts - 1) / parts; }
+        }
     } else {
         for (rsh = 0; rsh < 5 && (gpc << rsh) * 8 < GRAD_X_TURN * 5; ++rsh) {}
+        while (rsh > 0 && ctas() < 2ll * sm_count()) --rsh;
     }
-    while (rsh > 0 && (long long)((rows + (1 << rsh) - 1) >> rsh) * parts < 2ll * sm_count()) --rsh;
     grid = dim3((rows + (1 << rsh) - 1) >> rsh, (groups + gpc - 1) / gpc);
 }
 

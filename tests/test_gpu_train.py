@@ -1237,3 +1237,12 @@ def test_rows_on_both_sides_of_the_ctas_sizes(T, K, E, H, kind):
     test_permute(T, K, E, H, kind, 1)
     test_permute(T, K, E, H, kind, 4)
     test_restore(T, K, E, H, kind)
+
+
+@pytest.mark.parametrize("R,inner,kind", [(77, 4096, "bf16"), (3, 8320, "fp32"), (200, 4224, "fp16"), (591, 2048, "bf16"), (592, 2048, "fp32"), (1183, 1536, "bf16"),
+                                          (1186, 640, "fp32"), (2400, 640, "bf16"), (2367, 384, "fp16")])
+def test_swiglu_blocks_of_few_rows(R, inner, kind):
+    """Blocks that are halved, in rows or in groups, until there are four CTAs per SM, and those on the line."""
+    test_swiglu_save_of_several_turns(R, inner, kind, 1.0)
+    test_swiglu_save_of_several_turns(R, inner, kind, 0.87)
+    test_swiglu_backward(R, inner, kind, 0.87)
