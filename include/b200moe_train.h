@@ -69,7 +69,7 @@ int b200moe_combine_backward(const void* grad_out, const void* rows, int type, c
 /* SwiGLU of GEMM1's rows [num_rows, 2 * intermediate] (columns as the operator has them: act = rows[:, :I] * silu(rows[:, I:])), and the 8-bit
  * copy of the rows that the backward pass works from: q e4m3 [num_rows, 2I], scale float [2I / 128, num_rows], scale = the smallest
  * power of two not below amax / 448 of the 128 columns (at least 2^-126; 1 where all are zero; NaN where one is infinite or NaN;
- * codes end at 240 under the scale 2^120: a finite value is restored as a finite one).
+ * codes end at 240 under the scale 2^120: a finite value is restored as a finite one in fp32 and bf16; in fp16 one above 63488 is restored as an infinity).
  * used_rows: device pointer to the number of rows in use (expert_row0 + num_local), NULL = all; the others are left as they were.  Padding of the segments
  * is in use: it is taken like any row here and in the gradient, zeros give zeros, and what is not finite there stays so - the GEMMs around have to
  * leave zeros in it.  The sigmoid of a gate below -87 leaves fp32's

@@ -81,7 +81,7 @@ __device__ __forceinline__ void store_elems(T* dst, const float* v) {
 }
 
 // ---------------------------------------------------------------- sort
-// Latency: 56 pairs 2.5 us, 2048 5.7, 65536 6.5, 112856 (over 256 experts) 8.4, against 0.2 us of memory traffic at most.  One CTA for few
+// Latency: 56 pairs 2.5 us, 2048 5.8, 32768 6.1, 112856 (over 256 experts) 8.5, against 0.2 us of memory traffic at most.  One CTA for few
 // pairs, one meeting less than a kernel more; else two kernels, of which the second has ranked its pairs before it waits for the first.
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_ROUNDS = 4;                                 // pairs a thread holds
@@ -616,10 +616,13 @@ __device__ __forceinline__ void combine_grad_by_tokens(const OrderParams& o, con
     }
 }
 
-// By rows for few tokens, and where few of the picks have a row here (an expert-parallel rank's share).  By tokens / by rows, us, 7168
-// columns: one token 9.6 / 3.2, 64: 16 / 17, 256: 24 / 24, 512: 32 / 34, 2048: 90 / 97, 4096: 166 / 196, 8192: 322 / 409; 4096 tokens with one row each 61 /
-// 30, two 72 / 53, four 99 / 98 (CTAs of 256 threads).  Groups of 2^row_sh or 2^token_sh threads; with 256 threads per CTA, two tokens that wait for
-// each other in every turn, 512 tokens took 33.8 us (31.1 with 128), 4096: 165.9 (164.4).
+// By rows for few tokens, and where few of the picks have a row here (an expert-parallel rank's share).  By tokens / by rows, us, 8 picks of 256 experts, all
+// here: 7168 columns one token 8.6 / 2.6, 64: 17.1 / 17.1, 128: 19.5 / 19.9, 256: 22.6 / 22.7, 512: 31.4 / 32.8, 1024: 49.8 / 51.7, 4096: 165 / 195; 2048 columns 64:
+// 7.3 / 5.3, 256: 8.5 / 6.7, 512: 12.0 / 11.5, 1024: 16.3 / 18.2; 256 columns 256: 3.1 / 2.8, 512: 3.4 / 3.6, 1024: 3.9 / 5.4.
+// 4096 tokens with one / two / three / four rows each: 7168 columns 57 / 29, 69 / 50, 81 / 73, 95 / 95; 2048 columns 22 / 9, 26 / 16, 29 / 22, 33 / 28; 256 columns
+// 4.8 / 3.5, 5.2 / 5.3, 5.4 / 7.0, 5.8 / 9.4: a line (rows in use, padding counted) between what wide and narrow rows ask for.
+// Groups of 2^row_sh or 2^token_sh threads; with 256 threads per CTA, two tokens that wait for each other in every turn, 512 tokens took 33.8 us (31.1
+// with 128), 4096: 165.9 (164.4), 64, by rows, 17.6 (17.2).
 // In both ways all threads of a CTA make the same number of turns, as they meet in each; the sums' two buffers let a warp be one turn
 // ahead of the thread that reads them.
 constexpr int GRAD_FEW_TOKENS = 256, GRAD_FEW_ROWS = 3;

@@ -9,14 +9,15 @@
 // with 1 / scale is exact, so a code is x / scale rounded once, without a division, and the copy of 16-bit values is restored
 // without a rounding.  An e4m3 number has the same relative precision in the upper half of its range as at its end, so the copy loses
 // nothing to amax / 448 but one of the 15 binades above its subnormals.  Under the scale 2^120 the codes end at 240, so that no finite value is
-// restored as an infinity (off by less than 2^-4, like any other code).  A group that holds an infinity or a NaN gets the scale NaN: its values
+// an infinity in fp32 or bf16 when it is restored (off by less than 2^-4, like any other code).  In fp16 one above 63488, whose code stands for 65536, would be; the
+// gradient is made from the copy in fp32, where it is finite.  A group that holds an infinity or a NaN gets the scale NaN: its values
 // are gone, and the gradients made from it say so instead of being finite.
 // Byte work: 2048 columns of bf16, 34645 rows in use, save 88 us, backward with the activation 105 us in a row of such calls: 100 and 104 % of
-// the measured copy rate over the bytes that have to move; 8000 rows 23 and 26 us (88 and 96 %), 20000 rows of 256 columns 9.2 and 10 us.  The
-// arithmetic has to stay out of the way, also at the clocks of a long run under the power limit: products with powers of two instead of
-// divisions, two values per instruction, magnitudes compared two 16-bit patterns at a time, flushed approximations for 16-bit rows, no division in
-// the walk over a block.  With one value per instruction and the library's exponential and quotient the save kernel issued in 64 % of its cycles: 91 and
-// 110 us for short, 97 and 115 after a second of load (92 and 108 now).
+// the measured copy rate over the bytes that have to move (after a second of load 92 and 108, at the clocks of the power limit); without the activation 84; 8000 rows
+// 23 and 26 us (88 and 96 %), 20000 rows of 256 columns 9.0 and 9.8 us.  The arithmetic has to stay out of the way, also at those clocks: products with powers
+// of two instead of divisions, two values per instruction, magnitudes compared two 16-bit patterns at a time, flushed approximations for 16-bit rows, no
+// division in the walk over a block.  With one value per instruction and the library's exponential and quotient the save kernel issued in 64 % of its
+// cycles: 91 and 110 us for short, 97 and 115 after a second of load.
 #pragma once
 #include "order.cuh"
 

@@ -36,7 +36,7 @@ bool known_type(int type) { return type == B200MOE_TYPE_BF16 || type == B200MOE_
 int type_bytes(int type) { return type == B200MOE_TYPE_FP32 ? 4 : 2; }
 
 // Slices of a thread's one pair each, longer ones where that would be more CTAs than the chip holds at once (every CTA reads all slices'
-// histograms).  Up to SORT_ALONE pairs one CTA and one launch: 2048 pairs 5.9 us against 5.5 (and 4 us less of host time), 4096: 9.3 against 5.5.
+// histograms).  Up to SORT_ALONE pairs one CTA and one launch: 2048 pairs 5.8 us against 5.5 (and 4 us less of host time), 4096: 9.3 against 5.5.
 int sort_slice(int n) {
     const int most = 2 * sm_count();
     return ((n + most - 1) / most + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;

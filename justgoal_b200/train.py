@@ -35,6 +35,7 @@ from .inputs import ROUTING_DS
 from .main import _raw_stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_BYTES = (2, 2, 4)              # by the codes above
 _ALIGN = 32
 _I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
@@ -59,11 +60,12 @@ class TokenOrder(NamedTuple):
 
 
 def _call(fn, device, *args):
+    """fn(*args) with `device` current; the last argument is the device's current stream."""
     if _current_device() == device:
-        rc = fn(*args, _raw_stream(device))
+        rc = fn(*args)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device))
+            rc = fn(*args)
     if rc:
         _lib.check(rc, fn.__name__)
 
@@ -94,13 +96,13 @@ def _in(t, name, device, dtype, shape, align=1):
 
 def _rows(t, name, columns=128):
     """A row tensor that tells the call's type, device and sizes: (the tensor, its address, type, device, rows, columns)."""
-    kind = _TYPES.get(t.dtype)
-    if kind is None or t.dim() != 2:
-        raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
+    kind, shape = _TYPES.get(t.dtype), t.shape
+    if kind is None or len(shape) != 2:
+        raise ValueError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(shape)}")
     device = t.get_device()
     if device < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    n, H = t.shape
+    n, H = shape
     if H <= 0 or H % columns or H > columns << 13:
         raise ValueError(f"{name}: columns must be a multiple of {columns} up to {columns << 13}, got {H}")
     at = t.data_ptr()
@@ -110,16 +112,15 @@ def _rows(t, name, columns=128):
     return t, at, kind, device, n, H
 
 
-def _given(t, name, device, dtype, shape, align, *others):
-    """The address of the caller's output, which has to be of the form that is written in place and share no memory with the call's
-    inputs and other outputs (tensors, or addresses with their numbers of bytes)."""
+def _given(t, name, device, dtype, shape, size, align, *taken):
+    """The address of the caller's output of `size` bytes, which has to be of the form that is written in place and share no memory with the call's
+    inputs and other outputs (their addresses and ends)."""
     at = t.data_ptr()
     if t.dtype is not dtype or t.shape != shape or t.get_device() != device or at % align or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on cuda:{device} that starts at a multiple of {align} bytes")
-    end = at + t.nbytes
-    for other in others:
-        start, n = other if type(other) is tuple else (other.data_ptr(), other.nbytes)
-        if start < end and at < start + n and at < end:
+    end = at + size
+    for start, stop in taken:
+        if start < end and at < stop:
             raise ValueError(f"{name} must not share memory with an input or another output")
     return at
 
@@ -127,16 +128,19 @@ def _given(t, name, device, dtype, shape, align, *others):
 def _order(order, device):
     """An order's tables (kept by the caller until the call is made), their addresses, T, top_k, E_local, rows."""
     row0, row_pair, pair_row = order
-    if not (row0.dtype is _I32 and row_pair.dtype is _I32 and pair_row.dtype is _I32 and row0.dim() == 1 and row_pair.dim() == 1
-            and pair_row.dim() == 2 and row0.get_device() == device and row_pair.get_device() == device and pair_row.get_device() == device):
+    try:
+        (El,), (R,), (T, K) = row0.shape, row_pair.shape, pair_row.shape
+    except ValueError:                       # another number of dimensions
+        El = None
+    if not (El is not None and row0.dtype is _I32 and row_pair.dtype is _I32 and pair_row.dtype is _I32 and row0.get_device() == device
+            and row_pair.get_device() == device and pair_row.get_device() == device):
         raise ValueError(f"an order is int32 expert_row0 [E_local + 1], row_pair [max_rows] and pair_row [T, top_k] on cuda:{device}")
     if not (row0.is_contiguous() and row_pair.is_contiguous() and pair_row.is_contiguous()):
         order = row0, row_pair, pair_row = row0.contiguous(), row_pair.contiguous(), pair_row.contiguous()
-    T, K = pair_row.shape
-    El = row0.numel() - 1
+    El -= 1
     if not (1 <= El <= 512 and 1 <= K <= 8):
         raise ValueError("an order has 1 to 512 local experts and 1 to 8 picks per token")
-    return order, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T, K, El, row_pair.numel()
+    return order, row0.data_ptr(), row_pair.data_ptr(), pair_row.data_ptr(), T, K, El, R
 
 
 def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0, align: int = 16,
@@ -165,7 +169,7 @@ def sort_tokens(topk_idx: torch.Tensor, num_local_experts: int, local_expert_off
     pair_row = torch.empty_like(topk_idx)
     counts = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(_lib.lib.b200moe_sort_tokens, device, idx_at, T, K, El, local_expert_offset, align, rows, row0.data_ptr(), row_pair.data_ptr(),
-          pair_row.data_ptr(), None if counts is None else counts.data_ptr(), n)
+          pair_row.data_ptr(), None if counts is None else counts.data_ptr(), n, _raw_stream(device))
     return TokenOrder(row0, row_pair, pair_row)
 
 
@@ -180,8 +184,10 @@ def permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor] = No
         out = x.new_empty((R, H))
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, x.dtype, (R, H), _ALIGN, x, (row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
-    _call(_lib.lib.b200moe_permute, device, x_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
+        row = H * _BYTES[kind]
+        at = _given(out, "out", device, x.dtype, (R, H), R * row, _ALIGN, (x_at, x_at + T * row), (row0, row0 + 4 * El + 4),
+                    (row_pair, row_pair + 4 * R), (pair_row, pair_row + 4 * T * K))
+    _call(_lib.lib.b200moe_permute, device, x_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at, _raw_stream(device))
     if not made:
         _written(out)
     return out
@@ -198,8 +204,10 @@ def _combine(rows, w, order, out):
         out = rows.new_empty((T, H))
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, rows.dtype, (T, H), _ALIGN, rows, (pair_row, 4 * T * K), (w_at or 0, 0 if w is None else 4 * T * K))
-    _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row, T, K, H, R, at)
+        row = H * _BYTES[kind]
+        at = _given(out, "out", device, rows.dtype, (T, H), T * row, _ALIGN, (rows_at, rows_at + R * row), (pair_row, pair_row + 4 * T * K),
+                    (0, 0) if w is None else (w_at, w_at + 4 * T * K))
+    _call(_lib.lib.b200moe_combine, device, rows_at, kind, w_at, pair_row, T, K, H, R, at, _raw_stream(device))
     if not made:
         _written(out)
     return out
@@ -230,9 +238,12 @@ def combine_backward(grad_out: torch.Tensor, rows: torch.Tensor, topk_w: torch.T
         out = torch.empty_like(rows)
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, rows.dtype, (R, H), _ALIGN, rows, grad_out, topk_w, (row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
+        row = H * _BYTES[kind]
+        at = _given(out, "out", device, rows.dtype, (R, H), R * row, _ALIGN, (rows_at, rows_at + R * row), (grad_at, grad_at + T * row),
+                    (w_at, w_at + 4 * T * K), (row0, row0 + 4 * El + 4), (row_pair, row_pair + 4 * R), (pair_row, pair_row + 4 * T * K))
     grad_w = torch.empty_like(topk_w)
-    _call(_lib.lib.b200moe_combine_backward, device, grad_at, rows_at, kind, w_at, row0, row_pair, pair_row, T, K, El, H, R, at, grad_w.data_ptr())
+    _call(_lib.lib.b200moe_combine_backward, device, grad_at, rows_at, kind, w_at, row0, row_pair, pair_row, T, K, El, H, R, at, grad_w.data_ptr(),
+          _raw_stream(device))
     if not made:
         _written(out)
     return out, grad_w
@@ -267,23 +278,24 @@ def restore_1x128(q: torch.Tensor, scale: torch.Tensor, order: Optional[TokenOrd
         out = q.new_empty((R, H), dtype=dtype)
         at = out.data_ptr()
     else:
-        tables = () if order is None else ((row0, 4 * El + 4), (row_pair, 4 * R), (pair_row, 4 * T * K))
-        at = _given(out, "out", device, dtype, (R, H), _ALIGN, q, scale, *tables)
-    _call(_lib.lib.b200moe_restore_1x128, device, q_at, scale_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at)
+        tables = () if order is None else ((row0, row0 + 4 * El + 4), (row_pair, row_pair + 4 * R), (pair_row, pair_row + 4 * T * K))
+        at = _given(out, "out", device, dtype, (R, H), R * H * _BYTES[kind], _ALIGN, (q_at, q_at + T * H), (scale_at, scale_at + T * H // 32), *tables)
+    _call(_lib.lib.b200moe_restore_1x128, device, q_at, scale_at, kind, row0, row_pair, pair_row, T, K, El, H, R, at, _raw_stream(device))
     if not made:
         _written(out)
     return out
 
 
 def _used(expert_row0, device):
-    """(the table, kept by the caller until the call is made; the address of its last entry: the number of rows in use)"""
+    """(the table, kept by the caller until the call is made; its address and end; the address of its last entry: the number of rows in use)"""
     if expert_row0 is None:
-        return None, None
-    n = expert_row0.numel()
-    if expert_row0.dim() != 1 or n < 1:
+        return None, (0, 0), None
+    shape = expert_row0.shape
+    if len(shape) != 1 or shape[0] < 1:
         raise ValueError("expert_row0 must be int32 [E_local + 1]")
-    t, at = _in(expert_row0, "expert_row0", device, _I32, (n,))
-    return t, at + 4 * (n - 1)
+    t, at = _in(expert_row0, "expert_row0", device, _I32, shape)
+    end = at + 4 * shape[0]
+    return t, (at, end), end - 4
 
 
 def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = None, out=None):
@@ -292,18 +304,20 @@ def swiglu_save(gemm1_rows: torch.Tensor, expert_row0: Optional[torch.Tensor] = 
     magnitude / 448; one that holds an infinity or a NaN gets the scale NaN.  `expert_row0`: only its last entry's number of rows is in use (None:
     all).  `out`: the three tensors to write."""
     x, x_at, kind, device, R, I2 = _rows(gemm1_rows, "gemm1_rows", 256)
-    keep, used = _used(expert_row0, device)
+    keep, table, used = _used(expert_row0, device)
     if out is None:
         act, q = x.new_empty((R, I2 // 2)), x.new_empty((R, I2), dtype=_E4M3)
         scale = x.new_empty((I2 // 128, R), dtype=_F32)
         act_at, q_at, scale_at = act.data_ptr(), q.data_ptr(), scale.data_ptr()
     else:
         act, q, scale = out
-        ins = (x,) if keep is None else (x, keep)
-        act_at = _given(act, "act", device, x.dtype, (R, I2 // 2), _ALIGN, *ins)
-        q_at = _given(q, "q", device, _E4M3, (R, I2), 16, *ins, act)
-        scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), 4, *ins, act, q)
-    _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act_at, q_at, scale_at)
+        act_bytes, n = R * I2 // 2 * _BYTES[kind], R * I2
+        ins = (x_at, x_at + 2 * act_bytes)
+        act_at = _given(act, "act", device, x.dtype, (R, I2 // 2), act_bytes, _ALIGN, ins, table)
+        acts = (act_at, act_at + act_bytes)
+        q_at = _given(q, "q", device, _E4M3, (R, I2), n, 16, ins, table, acts)
+        scale_at = _given(scale, "scale", device, _F32, (I2 // 128, R), n // 32, 4, ins, table, acts, (q_at, q_at + n))
+    _call(_lib.lib.b200moe_swiglu_save, device, x_at, kind, used, R, I2 // 2, act_at, q_at, scale_at, _raw_stream(device))
     if out is not None:
         _written((act, q, scale))
     return act, q, scale
@@ -314,7 +328,7 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
     """Gradient of `swiglu_save`'s activation from its 8-bit copy: (grad of gemm1_rows [R, 2I], act [R, I] again or None), both of
     grad_act's type.  `out`: the two tensors to write (the second None without `with_act`)."""
     d, d_at, kind, device, R, I = _rows(grad_act, "grad_act")
-    keep, used = _used(expert_row0, device)
+    keep, table, used = _used(expert_row0, device)
     q, q_at = _in(q, "q", device, _E4M3, (R, 2 * I), 16)
     scale, scale_at = _in(scale, "scale", device, _F32, (2 * I // 128, R))
     if out is None:
@@ -324,10 +338,11 @@ def swiglu_backward(q: torch.Tensor, scale: torch.Tensor, grad_act: torch.Tensor
         grad_x, act = out
         if (act is not None) != with_act:
             raise ValueError("out has a tensor for act if and only if with_act asks for it")
-        ins = (q, scale, d) if keep is None else (q, scale, d, keep)
-        grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), _ALIGN, *ins)
-        act_at = _given(act, "act", device, d.dtype, (R, I), _ALIGN, *ins, grad_x) if with_act else None
-    _call(_lib.lib.b200moe_swiglu_backward, device, q_at, scale_at, d_at, kind, used, R, I, grad_at, act_at)
+        n = R * I * _BYTES[kind]
+        ins = (q_at, q_at + 2 * R * I), (scale_at, scale_at + R * I // 16), (d_at, d_at + n), table
+        grad_at = _given(grad_x, "grad_gemm1_rows", device, d.dtype, (R, 2 * I), 2 * n, _ALIGN, *ins)
+        act_at = _given(act, "act", device, d.dtype, (R, I), n, _ALIGN, *ins, (grad_at, grad_at + 2 * n)) if with_act else None
+    _call(_lib.lib.b200moe_swiglu_backward, device, q_at, scale_at, d_at, kind, used, R, I, grad_at, act_at, _raw_stream(device))
     if out is not None:
         _written((grad_x, act) if with_act else grad_x)
     return grad_x, act
@@ -355,8 +370,10 @@ def route_backward(routing_logits: torch.Tensor, routing_bias: Optional[torch.Te
         out = torch.empty_like(logits)
         at = out.data_ptr()
     else:
-        at = _given(out, "out", device, _F32, (T, E), 16, logits, grad_w, topk_idx, *(() if bias is None else (bias,)))
-    _call(_lib.lib.b200moe_route_backward, device, logits_at, bias_at, idx_at, grad_at, T, E, K, float(routed_scaling_factor), routing_mode, at)
+        at = _given(out, "out", device, _F32, (T, E), 4 * T * E, 16, (logits_at, logits_at + 4 * T * E), (idx_at, idx_at + 4 * T * K),
+                    (grad_at, grad_at + 4 * T * K), (0, 0) if bias is None else (bias_at, bias_at + 2 * E))
+    _call(_lib.lib.b200moe_route_backward, device, logits_at, bias_at, idx_at, grad_at, T, E, K, float(routed_scaling_factor), routing_mode, at,
+          _raw_stream(device))
     if not made:
         _written(out)
     return out

@@ -1246,3 +1246,19 @@ def test_swiglu_blocks_of_few_rows(R, inner, kind):
     test_swiglu_save_of_several_turns(R, inner, kind, 1.0)
     test_swiglu_save_of_several_turns(R, inner, kind, 0.87)
     test_swiglu_backward(R, inner, kind, 0.87)
+
+
+def test_fp16_rows_at_the_end_of_their_range():
+    """65504 has the code of 65536: finite in fp32 and bf16, an infinity where it is restored as fp16; the gradients, made in fp32, are finite."""
+    from justgoal_b200 import restore_1x128, swiglu_backward, swiglu_save
+    x = torch.full((2, 256), 65504.0, dtype=torch.float16)
+    x[:, 128:] = 0.5
+    x[1, :128] = -63488.0                                # (half-way, to the even code: 256)
+    x[1, 1:128] = -63456.0                               # ... and the next smaller: 240
+    _, q, scale = swiglu_save(x.cuda())
+    for dtype in (torch.float32, torch.bfloat16):
+        back = restore_1x128(q, scale, dtype=dtype)
+        assert bool((back[0, :128] == 65536).all()) and float(back[1, 0]) == -65536 and bool((back[1, 1:128] == -61440).all())
+    assert bool(restore_1x128(q, scale, dtype=torch.float16)[0, :128].isinf().all())
+    grad, act = swiglu_backward(q, scale, torch.full((2, 128), 1e-3, dtype=torch.float16, device="cuda"))
+    assert bool(torch.isfinite(grad).all()) and bool(torch.isfinite(act).all())

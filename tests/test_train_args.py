@@ -137,3 +137,18 @@ def test_sort_workspace_of_a_size_is_enough_for_smaller_ones():
         assert by_experts == sorted(by_experts)
     pairs = [size(T, K=1) for T in range(2000, 320000, 333)]
     assert pairs == sorted(pairs)
+
+
+@pytest.mark.parametrize("tables", [((2, 33), (100,), (4, 8)), ((33,), (100, 1), (4, 8)), ((33,), (100,), (32,)), ((33,), (100,), (4, 8, 1)), ((), (100,), (4, 8)),
+                                    ((33,), (), (4, 8)), ((0,), (100,), (4, 8)), ((1,), (100,), (4, 8)), ((33,), (100,), (4, 9)), ((33,), (100,), (4, 0)), ((514,), (100,), (4, 8))])
+def test_orders_of_other_forms_are_refused(tables):
+    """Tables of another number of dimensions, of no or too many experts or picks (the check itself, which takes the device's number: -1 is the host)."""
+    from justgoal_b200.train import _order
+    make = lambda shapes, dtype=torch.int32: [torch.zeros(s, dtype=dtype) for s in shapes]   # noqa: E731
+    assert _order(make(((33,), (100,), (4, 8))), -1)[4:] == (4, 8, 32, 100)
+    with pytest.raises(ValueError, match="an order"):
+        _order(make(tables), -1)
+    with pytest.raises(ValueError, match="an order is int32"):
+        _order(make(((33,), (100,), (4, 8)), torch.int64), -1)
+    with pytest.raises(ValueError, match="an order is int32"):
+        _order(make(((33,), (100,), (4, 8))), 0)
