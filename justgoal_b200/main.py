@@ -240,9 +240,8 @@ class MoELayer:
             raise ValueError("topk_idx int32, topk_w float32, send_token int64")
         wire = torch.empty(n, self.ep_row_bytes(), dtype=torch.uint8, device=hidden_states.device)
         stream = torch.cuda.current_stream(hidden_states.device).cuda_stream
-        rc = _lib.lib.b200moe_ep_pack(self._h, _ptr(_contig(hidden_states)), _ptr(_contig(hidden_states_scale)),
-                                      _ptr(_contig(topk_idx)), _ptr(_contig(topk_w)), _ptr(_contig(send_token)), n, T,
-                                      _ptr(wire), C.c_void_p(stream))
+        tensors = [_contig(t) for t in (hidden_states, hidden_states_scale, topk_idx, topk_w, send_token)]   # copies live until the call
+        rc = _lib.lib.b200moe_ep_pack(self._h, *[_ptr(t) for t in tensors], n, T, _ptr(wire), C.c_void_p(stream))
         _lib.check(rc, "b200moe_ep_pack")
         return wire
 
@@ -268,8 +267,9 @@ class MoELayer:
             raise ValueError("partial_rows must be fp16 [n, hidden] and row_of int32 [world, T]")
         out = torch.empty(num_tokens, s.hidden, dtype=torch.bfloat16, device=partial_rows.device)
         stream = torch.cuda.current_stream(partial_rows.device).cuda_stream
-        rc = _lib.lib.b200moe_ep_combine(self._h, _ptr(_contig(partial_rows)), _ptr(_contig(row_of)), world,
-                                         int(num_tokens), _ptr(out), C.c_void_p(stream))
+        partial_rows, row_of = _contig(partial_rows), _contig(row_of)
+        rc = _lib.lib.b200moe_ep_combine(self._h, _ptr(partial_rows), _ptr(row_of), world, int(num_tokens), _ptr(out),
+                                         C.c_void_p(stream))
         _lib.check(rc, "b200moe_ep_combine")
         return out
 
@@ -306,7 +306,8 @@ class MoELayer:
         if expert_row0.numel() < self.shape.num_local_experts + 1:
             raise ValueError("expert_row0 needs num_local_experts + 1 entries")
         stream = torch.cuda.current_stream(dev).cuda_stream
-        rc = _lib.lib.b200moe_permute_noalloc(self._h, _ptr(_contig(topk_idx)), _ptr(_contig(topk_w)), T,
+        topk_idx, topk_w = _contig(topk_idx), _contig(topk_w)
+        rc = _lib.lib.b200moe_permute_noalloc(self._h, _ptr(topk_idx), _ptr(topk_w), T,
                                               _scalar(local_expert_offset, int), _ptr(expert_row0),
                                               _ptr(row_token), _ptr(row_w), min(int(row_token.numel()), int(row_w.numel())),
                                               C.c_void_p(stream))
