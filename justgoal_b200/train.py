@@ -19,8 +19,9 @@ counts in `sort_tokens`), keeps nothing, and can be captured into a CUDA graph. 
 not start at a 32-byte boundary, are copied first (`out` tensors are refused).  Row tensors have room for `order.row_pair.numel()` rows:
 `permute`, `restore_1x128` and `combine_backward` write the rows in use, padding of the segments included (as zeros).  The SwiGLU pair takes padding for
 rows like any other: zeros give zeros, but what a GEMM leaves unset there comes out as whatever it makes, so GEMMs have to write zeros into it (from the
-zeros that they read).  All of them leave rows behind `expert_row0[-1]` as they were (unset where the call makes the tensor).  The gradients are plain functions: autograd does not record these calls.  A call that
-writes an `out` tensor counts as a change of it in place: a backward pass that had saved it raises, as after any change in place.
+zeros that they read).  All of them leave rows behind `expert_row0[-1]` as they were (unset where the call makes the tensor).  The gradients are plain
+functions: autograd does not record these calls.  A call that writes an `out` tensor counts as a change of it in place: a backward pass that had saved
+it raises, as after any change in place.
 """
 from __future__ import annotations
 
